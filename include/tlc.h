@@ -64,6 +64,17 @@ typedef struct tlc_tensor {
     int64_t strides[TLC_MAX_DIMS];
 } tlc_tensor;
 
+/* A strided view of token numbers (or any other index): `bits` is 32 or 64
+ * (int32_t or int64_t elements), strides in elements.  The reference's tensors
+ * are floats alone; this is what goes into tlc_embedding and its kin. */
+typedef struct tlc_index {
+    void* data;
+    int32_t ndim;
+    int32_t bits;
+    int64_t sizes[TLC_MAX_DIMS];
+    int64_t strides[TLC_MAX_DIMS];
+} tlc_index;
+
 /* One batched, strided GEMM: for every batch index b (up to 3 batch dims,
  * row-major order), C_b[m,n] = sum_k A_b[m,k] * B_b[k,n] with
  *   A_b[m,k] = A[off_a(b) + m*a_rs + k*a_cs]     (a_cs == 1: row-major A;
@@ -303,6 +314,77 @@ int tlc_flash_attention_backward(const tlc_tensor* grad_out, const tlc_tensor* q
                                  const tlc_tensor* k, const tlc_tensor* v, const tlc_tensor* out,
                                  const tlc_tensor* lse, float sm_scale, tlc_tensor* d_q,
                                  tlc_tensor* d_k, tlc_tensor* d_v, int mode, void* stream);
+
+/* ---- token models: the parts around Linear and attention -----------------------
+ * Layer norm, embedding lookup and token log-probabilities with their
+ * gradients, fp32 (the reference has nn::LayerNorm, nn::Embedding and
+ * cross-entropy on the CPU, nn.h:56-630 and loss.cpp:12-103; these follow the
+ * formulas, not its order of additions: sums are trees in fp32).
+ * Inputs are any views with strides >= 0 (a view whose last dim has stride 1 is
+ * read in place, any other is copied first); outputs are contiguous, are
+ * overwritten unless said otherwise, and may not lie over inputs or each other
+ * (TLC_ERR_INVALID_ARGUMENT).  Results are the same bits on every call.
+ * Shapes that differ, strides, NULL or misaligned data: TLC_ERR_INVALID_ARGUMENT,
+ * before anything is launched.  All of it can be captured into a CUDA graph. */
+
+/* y = (x - mean) rstd * weight + bias over the last dim D of x, with
+ * rstd = 1 / sqrt(var + eps) and var = sum (x - mean)^2 / D.  weight and bias:
+ * NULL or [D].  stats: NULL or [..., 2], receives (mean, rstd) of each row:
+ * what the backward needs.  eps must be finite and >= 0. */
+int tlc_layer_norm(const tlc_tensor* x, const tlc_tensor* weight, const tlc_tensor* bias, float eps,
+                   tlc_tensor* out, tlc_tensor* stats, void* stream);
+/* The gradients from grad (x's shape), x, the forward's stats and weight
+ * (NULL: 1): with xhat = (x - mean) rstd and gw = grad * weight,
+ *   dx = rstd (gw - mean(gw) - xhat mean(gw xhat)),
+ *   dweight = sum over rows of grad xhat,  dbias = sum over rows of grad.
+ * NULL skips one.  accumulate != 0 adds to what the outputs hold (as
+ * tlc_matmul_backward does; for dx, a residual branch's gradient). */
+int tlc_layer_norm_backward(const tlc_tensor* grad, const tlc_tensor* x, const tlc_tensor* stats,
+                            const tlc_tensor* weight, tlc_tensor* dx, tlc_tensor* dweight,
+                            tlc_tensor* dbias, int accumulate, void* stream);
+
+/* out[i] = scale * weight[tokens[i]]: weight [V, D], tokens of any shape (at
+ * most 7 dims), out [tokens' shape, D].  A token of -1 is padding: a row of
+ * zeros.  Any other token outside [0, V) gives a row of NaN (nothing outside
+ * `weight` is read). */
+int tlc_embedding(const tlc_tensor* weight, const tlc_index* tokens, float scale, tlc_tensor* out,
+                  void* stream);
+/* dweight[v] = scale * sum of grad[i] over the positions with tokens[i] == v,
+ * zeros for tokens that do not occur; with accumulate != 0 these sums are
+ * added to what dweight holds (rows that do not occur stay as they are).
+ * Tokens outside [0, V), -1 among them, take no part.  The positions are
+ * sorted by token, so each row's additions have one fixed order. */
+int tlc_embedding_backward(const tlc_tensor* grad, const tlc_index* tokens, float scale,
+                           tlc_tensor* dweight, int accumulate, void* stream);
+
+/* For each row of logits [..., V] with p = softmax(scale * logits):
+ *   logprobs [...]: log p[token], tokens of logits' leading shape;
+ *   entropy [...]: -sum p log p;
+ *   stats [..., 2]: the row's largest logit m and log sum exp(scale (x - m)),
+ *     what the backward needs;
+ *   top_logprobs, top_tokens [..., top]: the `top` most likely tokens in
+ *     order, equal logits by the lower token, with their log p.
+ * Each output may be NULL (tokens too without logprobs; the two top_ ones
+ * exactly when top is 0).  0 <= top <= min(V, 32), above 32
+ * TLC_ERR_UNSUPPORTED; scale must be finite and > 0.
+ * Token -1: none is asked for, logprobs 0 (the row's other results as usual);
+ * any other token outside [0, V): NaN.  A row of -inf alone has no
+ * distribution: log-probabilities -inf, entropy 0.  A NaN or +inf in a row
+ * makes its results NaN; NaN ranks above every number in top_tokens. */
+int tlc_token_logprobs(const tlc_tensor* logits, const tlc_index* tokens, float scale,
+                       tlc_tensor* logprobs, tlc_tensor* entropy, tlc_tensor* stats, int top,
+                       tlc_tensor* top_logprobs, tlc_index* top_tokens, void* stream);
+/* The gradient to the logits from those of logprobs and entropy (NULL: none):
+ *   dlogits_j = scale (g (1[j = token] - p_j) - h p_j (log p_j + entropy)),
+ * with the forward's stats and, with grad_entropy, its entropy.  The gradients
+ * may be broadcast views (stride 0).  No gradient flows from top_logprobs, from
+ * the log-probability of token -1, or into a row of -inf alone; a token that
+ * gave NaN gives a row of NaN.  dlogits may be the memory of (contiguous)
+ * logits. */
+int tlc_token_logprobs_backward(const tlc_tensor* logits, const tlc_index* tokens,
+                                const tlc_tensor* stats, const tlc_tensor* entropy,
+                                const tlc_tensor* grad_logprobs, const tlc_tensor* grad_entropy,
+                                float scale, tlc_tensor* dlogits, void* stream);
 
 /* ---- TLMD model files straight to / from device memory --------------------
  * load_model / save_model (src/model_io.cpp:7-94): "TLMD", int32 version 1,

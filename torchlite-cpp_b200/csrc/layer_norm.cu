@@ -1,0 +1,560 @@
+// Layer norm over the last dim of [..., D] and its gradients, fp32.
+//
+//   mean = sum_D x / D,  var = sum_D (x - mean)^2 / D,  rstd = 1 / sqrt(var + eps)
+//   xhat = (x - mean) rstd,  y = xhat w + b
+//   dx = rstd (gw - (sum_D gw + xhat sum_D gw xhat) / D)   with gw = g w
+//   dw = sum_rows g xhat,  db = sum_rows g
+//
+// Bound by HBM: the forward moves 8 bytes an element (x in, y out), the
+// backward 12 (x and g in, dx out).  So a row is read once, into registers,
+// and both statistics come from there (the mean first, then the squares of
+// the differences: no cancellation).
+#include <algorithm>
+#include <cmath>
+
+#include "rows.cuh"
+
+namespace tlc {
+namespace {
+
+struct LnFwd {
+    const float *x, *w, *b;
+    float *out, *stats;
+    Rows xm;
+    int64_t rows;
+    int D;
+    float eps;
+};
+
+// THREADS threads a row (32: a warp for each row, 4 rows a block), VPT vectors
+// of VEC floats a thread: D <= THREADS * VPT * VEC.
+template <int VEC, int VPT, int THREADS>
+__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) ln_fwd_kernel(LnFwd p) {
+    constexpr int RPB = THREADS == 32 ? 4 : 1;
+    __shared__ float red[2][32];
+    const int t = THREADS == 32 ? (threadIdx.x & 31) : threadIdx.x;
+    const int sub = THREADS == 32 ? (threadIdx.x >> 5) : 0;
+    for (int64_t r = (int64_t)blockIdx.x * RPB + sub; r < p.rows; r += (int64_t)gridDim.x * RPB) {
+        const float* xr = p.x + p.xm.offset(r);
+        float v[VPT][VEC];
+        float s[1] = {0.0f};
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int j = (t + i * THREADS) * VEC;
+            if (j < p.D) {
+                load_once<VEC>(xr + j, v[i]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[i][k] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) s[0] += v[i][k];
+        group_sum<THREADS>(s, red[0]);
+        const float mean = __fdiv_rn(s[0], (float)p.D);  // exact for rows of one value
+        float q[1] = {0.0f};
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const bool in = (t + i * THREADS) * VEC < p.D;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                v[i][k] -= mean;
+                if (in) q[0] = fmaf(v[i][k], v[i][k], q[0]);
+            }
+        }
+        group_sum<THREADS>(q, red[1]);
+        const float rstd = __frsqrt_rn(__fdiv_rn(q[0], (float)p.D) + p.eps);
+        float* yr = p.out + r * p.D;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int j = (t + i * THREADS) * VEC;
+            if (j < p.D) {
+                float wv[VEC], bv[VEC], y[VEC];
+                if (p.w) load_vec<VEC>(p.w + j, wv);
+                if (p.b) load_vec<VEC>(p.b + j, bv);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    y[k] = v[i][k] * rstd;
+                    if (p.w) y[k] *= wv[k];
+                    if (p.b) y[k] += bv[k];
+                }
+                store_vec<VEC>(yr + j, y);
+            }
+        }
+        if (p.stats && t == 0) {
+            p.stats[2 * r] = mean;
+            p.stats[2 * r + 1] = rstd;
+        }
+    }
+}
+
+// Rows too long for the registers of a block: the row is read three times
+// (from L2 after the first).
+__global__ void __launch_bounds__(1024) ln_fwd_long_kernel(LnFwd p) {
+    __shared__ float red[2][32];
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const float* xr = p.x + p.xm.offset(r);
+        float s[1] = {0.0f};
+        for (int64_t j = threadIdx.x; j < p.D; j += 1024) s[0] += xr[j];
+        group_sum<1024>(s, red[0]);
+        const float mean = __fdiv_rn(s[0], (float)p.D);  // exact for rows of one value
+        float q[1] = {0.0f};
+        for (int64_t j = threadIdx.x; j < p.D; j += 1024) {
+            const float d = xr[j] - mean;
+            q[0] = fmaf(d, d, q[0]);
+        }
+        group_sum<1024>(q, red[1]);
+        const float rstd = __frsqrt_rn(__fdiv_rn(q[0], (float)p.D) + p.eps);
+        float* yr = p.out + r * p.D;
+        for (int64_t j = threadIdx.x; j < p.D; j += 1024) {
+            float y = (xr[j] - mean) * rstd;
+            if (p.w) y *= p.w[j];
+            if (p.b) y += p.b[j];
+            yr[j] = y;
+        }
+        if (p.stats && threadIdx.x == 0) {
+            p.stats[2 * r] = mean;
+            p.stats[2 * r + 1] = rstd;
+        }
+    }
+}
+
+struct LnBwd {
+    const float *g, *x, *w, *stats;
+    float *dx, *part;  // part: [gridDim.x][2][D], the blocks' sums for dw and db, or NULL
+    Rows gm, xm, sm;   // sm: the rows of stats
+    int64_t rows;
+    int D;
+    int accumulate;
+};
+
+// As the forward; each thread keeps the same columns for every row of its
+// block, so the sums for dw and db stay in its registers until the end.
+template <int VEC, int VPT, int THREADS>
+__global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) ln_bwd_kernel(LnBwd p) {
+    constexpr int RPB = THREADS == 32 ? 8 : 1;
+    extern __shared__ float sums[];  // THREADS == 32: [8][2][D]
+    __shared__ float red[2][64];
+    const int t = THREADS == 32 ? (threadIdx.x & 31) : threadIdx.x;
+    const int sub = THREADS == 32 ? (threadIdx.x >> 5) : 0;
+    const float inv = 1.0f / (float)p.D;
+    float aw[VPT][VEC], ab[VPT][VEC];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) aw[i][k] = ab[i][k] = 0.0f;
+    int turn = 0;
+    for (int64_t r = (int64_t)blockIdx.x * RPB + sub; r < p.rows; r += (int64_t)gridDim.x * RPB) {
+        const float* xr = p.x + p.xm.offset(r);
+        const float* gr = p.g + p.gm.offset(r);
+        const float* st = p.stats + p.sm.offset(r);
+        const float mean = st[0], rstd = st[1];
+        float x[VPT][VEC], g[VPT][VEC];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int j = (t + i * THREADS) * VEC;
+            if (j < p.D) {
+                load_once<VEC>(xr + j, x[i]);
+                load_once<VEC>(gr + j, g[i]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) x[i][k] = mean, g[i][k] = 0.0f;
+            }
+        }
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int j = (t + i * THREADS) * VEC;
+            float wv[VEC];
+            if (p.w && j < p.D) load_vec<VEC>(p.w + j, wv);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                x[i][k] = (x[i][k] - mean) * rstd;
+                aw[i][k] = fmaf(g[i][k], x[i][k], aw[i][k]);
+                ab[i][k] += g[i][k];
+                if (p.w && j < p.D) g[i][k] *= wv[k];
+                s[0] += g[i][k];
+                s[1] = fmaf(g[i][k], x[i][k], s[1]);
+            }
+        }
+        if (p.dx) {
+            group_sum<THREADS>(s, red[turn]);
+            turn ^= 1;
+            const float c0 = s[0] * inv, c1 = s[1] * inv;
+            float* dr = p.dx + r * p.D;
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int j = (t + i * THREADS) * VEC;
+                if (j < p.D) {
+                    float y[VEC], old[VEC];
+                    if (p.accumulate) load_vec<VEC>(dr + j, old);
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) {
+                        y[k] = __fmul_rn(rstd, g[i][k] - fmaf(x[i][k], c1, c0));
+                        if (p.accumulate) y[k] = __fadd_rn(y[k], old[k]);  // the gradient rounded, then added
+                    }
+                    store_vec<VEC>(dr + j, y);
+                }
+            }
+        }
+    }
+    if (!p.part) return;
+    float* part = p.part + (int64_t)blockIdx.x * 2 * p.D;
+    if constexpr (THREADS == 32) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int j = (t + i * THREADS) * VEC;
+            if (j < p.D) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    sums[(2 * sub) * p.D + j + k] = aw[i][k];
+                    sums[(2 * sub + 1) * p.D + j + k] = ab[i][k];
+                }
+            }
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < 2 * p.D; j += blockDim.x) {
+            float a = 0.0f;
+#pragma unroll
+            for (int q = 0; q < RPB; ++q) a += sums[q * 2 * p.D + j];
+            part[j] = a;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int j = (t + i * THREADS) * VEC;
+            if (j < p.D) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    part[j + k] = aw[i][k];
+                    part[p.D + j + k] = ab[i][k];
+                }
+            }
+        }
+    }
+}
+
+// Rows too long for that: dx alone, the row read twice ...
+__global__ void __launch_bounds__(1024) ln_bwd_long_kernel(LnBwd p) {
+    __shared__ float red[2][64];
+    const float inv = 1.0f / (float)p.D;
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const float* xr = p.x + p.xm.offset(r);
+        const float* gr = p.g + p.gm.offset(r);
+        const float* st = p.stats + p.sm.offset(r);
+        const float mean = st[0], rstd = st[1];
+        float s[2] = {0.0f, 0.0f};
+        for (int64_t j = threadIdx.x; j < p.D; j += 1024) {
+            const float gw = p.w ? gr[j] * p.w[j] : gr[j];
+            s[0] += gw;
+            s[1] = fmaf(gw, (xr[j] - mean) * rstd, s[1]);
+        }
+        group_sum<1024>(s, red[turn]);
+        turn ^= 1;
+        const float c0 = s[0] * inv, c1 = s[1] * inv;
+        float* dr = p.dx + r * p.D;
+        for (int64_t j = threadIdx.x; j < p.D; j += 1024) {
+            const float gw = p.w ? gr[j] * p.w[j] : gr[j];
+            float y = __fmul_rn(rstd, gw - fmaf((xr[j] - mean) * rstd, c1, c0));
+            if (p.accumulate) y = __fadd_rn(y, dr[j]);
+            dr[j] = y;
+        }
+    }
+}
+
+// ... and the columns' sums over a run of rows for each block row.
+__global__ void __launch_bounds__(256) ln_bwd_cols_kernel(LnBwd p, int64_t rows_per) {
+    const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (j >= p.D) return;
+    const int64_t r0 = blockIdx.y * rows_per, r1 = min(p.rows, r0 + rows_per);
+    float a = 0.0f, b = 0.0f;
+    for (int64_t r = r0; r < r1; ++r) {
+        const float* st = p.stats + p.sm.offset(r);
+        const float g = p.g[p.gm.offset(r) + j];
+        a = fmaf(g, (p.x[p.xm.offset(r) + j] - st[0]) * st[1], a);
+        b += g;
+    }
+    float* part = p.part + (int64_t)blockIdx.y * 2 * p.D;
+    part[j] = a;
+    part[p.D + j] = b;
+}
+
+// dw = sum of the blocks' sums in their order: 32 columns a block, 8 warps
+// over the parts.  Columns [0, D) are dw's, [D, 2D) db's.
+__global__ void __launch_bounds__(256) ln_bwd_finish_kernel(const float* __restrict__ part, int parts, int D,
+                                                            float* dw, float* db, int accumulate) {
+    __shared__ float red[8][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t j = (int64_t)blockIdx.x * 32 + lane;
+    float a = 0.0f;
+    if (j < 2 * (int64_t)D)
+        for (int q = warp; q < parts; q += 8) a += part[(int64_t)q * 2 * D + j];
+    red[warp][lane] = a;
+    __syncthreads();
+    if (warp == 0 && j < 2 * (int64_t)D) {
+        a = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) a += red[q][lane];
+        float* out = j < D ? (dw ? dw + j : nullptr) : (db ? db + (j - D) : nullptr);
+        if (out) *out = accumulate ? *out + a : a;
+    }
+}
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+        return 148;
+    return sms;
+}
+
+constexpr const char* kFwd = "layer_norm";
+constexpr const char* kBwd = "layer_norm_backward";
+
+template <int VEC, int VPT, int THREADS>
+int launch_fwd(const LnFwd& p, cudaStream_t s) {
+    constexpr int RPB = THREADS == 32 ? 4 : 1;
+    const int64_t want = (p.rows + RPB - 1) / RPB;
+    const unsigned grid = (unsigned)std::min<int64_t>(want, INT32_MAX);
+    ln_fwd_kernel<VEC, VPT, THREADS><<<grid, THREADS == 32 ? 128 : THREADS, 0, s>>>(p);
+    count_launch();
+    return check_launch(kFwd);
+}
+
+template <int VEC>
+int pick_fwd(const LnFwd& p, cudaStream_t s) {
+    const int n = (p.D + VEC - 1) / VEC;  // vectors a row
+    if (VEC * n <= 1024) {
+        if (n <= 32) return launch_fwd<VEC, 1, 32>(p, s);
+        if (n <= 64) return launch_fwd<VEC, 2, 32>(p, s);
+        if (n <= 128) return launch_fwd<VEC, 4, 32>(p, s);
+        if (n <= 192) return launch_fwd<VEC, 6, 32>(p, s);
+        if (n <= 256) return launch_fwd<VEC, 8, 32>(p, s);
+        if constexpr (VEC == 1) {
+            if (n <= 512) return launch_fwd<VEC, 16, 32>(p, s);
+            return launch_fwd<VEC, 32, 32>(p, s);
+        }
+    }
+    if (n <= 256 * 2) return launch_fwd<VEC, 2, 256>(p, s);
+    if (n <= 256 * 4) return launch_fwd<VEC, 4, 256>(p, s);
+    if (n <= 512 * 4) return launch_fwd<VEC, 4, 512>(p, s);
+    if (n <= 1024 * 4) return launch_fwd<VEC, 4, 1024>(p, s);
+    if constexpr (VEC == 1) {
+        if (n <= 1024 * 8) return launch_fwd<VEC, 8, 1024>(p, s);
+        if (n <= 1024 * 16) return launch_fwd<VEC, 16, 1024>(p, s);
+    }
+    ln_fwd_long_kernel<<<(unsigned)std::min<int64_t>(p.rows, INT32_MAX), 1024, 0, s>>>(p);
+    count_launch();
+    return check_launch(kFwd);
+}
+
+template <int VEC, int VPT, int THREADS>
+int launch_bwd(const LnBwd& p, int grid, cudaStream_t s) {
+    const size_t smem = THREADS == 32 && p.part ? sizeof(float) * 16 * (size_t)p.D : 0;
+    static DeviceOnce once;
+    if (smem)
+        TLC_TRY(smem_limit_once(once, ln_bwd_kernel<VEC, VPT, THREADS>, (int)(sizeof(float) * 16 * 1024)));
+    ln_bwd_kernel<VEC, VPT, THREADS><<<grid, THREADS == 32 ? 256 : THREADS, smem, s>>>(p);
+    count_launch();
+    return check_launch(kBwd);
+}
+
+// The rows a block of the register kernels takes at once (0: the row is too long).
+int bwd_threads(int D, int vec) {
+    const int n = (D + vec - 1) / vec;
+    if (n * vec <= (vec == 4 ? 1024 : 512)) return 32;
+    const int per = vec == 4 ? 4 : 16;
+    if (n <= 128 * per) return 128;
+    if (n <= 256 * per) return 256;
+    if (n <= 512 * per) return 512;
+    return 0;
+}
+
+template <int VEC>
+int pick_bwd(const LnBwd& p, int threads, int grid, cudaStream_t s) {
+    const int n = (p.D + VEC - 1) / VEC;
+    constexpr int PER = VEC == 4 ? 4 : 16;
+    if (threads == 32) {
+        if (n <= 32) return launch_bwd<VEC, 1, 32>(p, grid, s);
+        if (n <= 64) return launch_bwd<VEC, 2, 32>(p, grid, s);
+        if (n <= 128) return launch_bwd<VEC, 4, 32>(p, grid, s);
+        if constexpr (VEC == 4) {
+            if (n <= 192) return launch_bwd<VEC, 6, 32>(p, grid, s);
+            return launch_bwd<VEC, 8, 32>(p, grid, s);
+        } else {
+            if (n <= 256) return launch_bwd<VEC, 8, 32>(p, grid, s);
+            return launch_bwd<VEC, 16, 32>(p, grid, s);
+        }
+    }
+    if (threads == 128) return launch_bwd<VEC, PER, 128>(p, grid, s);
+    if (threads == 256) return launch_bwd<VEC, PER, 256>(p, grid, s);
+    return launch_bwd<VEC, PER, 512>(p, grid, s);
+}
+
+// A weight or bias: NULL, or a 1-D tensor of length D with stride 1 (a copy in `sc` otherwise).
+int column_vector(const tlc_tensor* t, const char* op, const char* name, int64_t D, RowScratch& sc, const float** out,
+                  Extent* ext) {
+    *out = nullptr;
+    if (!t) return TLC_OK;
+    TLC_TRY(shaped(t, op, name, 1, &D, false, ext));
+    RowView v;
+    TLC_TRY(row_view(t, op, name, v));
+    TLC_TRY(unit_rows(t, v, sc));
+    *out = v.data;
+    return TLC_OK;
+}
+
+}  // namespace
+}  // namespace tlc
+
+using namespace tlc;
+
+extern "C" int tlc_layer_norm(const tlc_tensor* x, const tlc_tensor* weight, const tlc_tensor* bias, float eps,
+                              tlc_tensor* out, tlc_tensor* stats, void* stream) {
+    clear_error();
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    RowView vx;
+    TLC_TRY(row_view(x, kFwd, "x", vx));
+    if (!(eps >= 0.0f) || std::isinf(eps))
+        return set_error(TLC_ERR_INVALID_ARGUMENT, "layer_norm: eps must be finite and not negative");
+    if (vx.cols > INT32_MAX / 4) return set_error(TLC_ERR_UNSUPPORTED, "layer_norm: last dim too large");
+    Extent eo, es, ew, eb;
+    TLC_TRY(shaped(out, kFwd, "out", x->ndim, x->sizes, true, &eo));
+    TLC_TRY(no_overlap(kFwd, "out", eo, "x", vx.ext));
+    if (stats) {
+        int64_t sz[TLC_MAX_DIMS];
+        std::copy(x->sizes, x->sizes + x->ndim, sz);
+        sz[x->ndim - 1] = 2;
+        TLC_TRY(shaped(stats, kFwd, "stats", x->ndim, sz, true, &es));
+        TLC_TRY(no_overlap(kFwd, "stats", es, "x", vx.ext));
+        TLC_TRY(no_overlap(kFwd, "stats", es, "out", eo));
+    }
+    if (weight) {
+        TLC_TRY(shaped(weight, kFwd, "weight", 1, &vx.cols, false, &ew));
+        TLC_TRY(no_overlap(kFwd, "out", eo, "weight", ew));
+        TLC_TRY(no_overlap(kFwd, "stats", es, "weight", ew));
+    }
+    if (bias) {
+        TLC_TRY(shaped(bias, kFwd, "bias", 1, &vx.cols, false, &eb));
+        TLC_TRY(no_overlap(kFwd, "out", eo, "bias", eb));
+        TLC_TRY(no_overlap(kFwd, "stats", es, "bias", eb));
+    }
+    if (vx.cols == 0 && vx.rows > 0 && stats)
+        return set_error(TLC_ERR_INVALID_ARGUMENT, "layer_norm: no statistics of rows without elements");
+    if (vx.numel == 0) return TLC_OK;
+    RowScratch cx(s), cw(s), cb(s);
+    TLC_TRY(unit_rows(x, vx, cx));
+    LnFwd p{};
+    TLC_TRY(column_vector(weight, kFwd, "weight", vx.cols, cw, &p.w, &ew));
+    TLC_TRY(column_vector(bias, kFwd, "bias", vx.cols, cb, &p.b, &eb));
+    p.x = vx.data;
+    p.xm = vx.map;
+    p.out = out->data;
+    p.stats = stats ? stats->data : nullptr;
+    p.rows = vx.rows;
+    p.D = (int)vx.cols;
+    p.eps = eps;
+    // float4 where every row of x, out, weight and bias starts on 16 bytes
+    const bool vec = p.D % 4 == 0 && vx.map.multiple_of(4) && aligned_to(p.x, 16) && aligned_to(p.out, 16) &&
+                     aligned_to(p.w, 16) && aligned_to(p.b, 16);
+    return vec ? pick_fwd<4>(p, s) : pick_fwd<1>(p, s);
+}
+
+extern "C" int tlc_layer_norm_backward(const tlc_tensor* grad, const tlc_tensor* x, const tlc_tensor* stats,
+                                       const tlc_tensor* weight, tlc_tensor* dx, tlc_tensor* dweight,
+                                       tlc_tensor* dbias, int accumulate, void* stream) {
+    clear_error();
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    RowView vx, vg, vs;
+    TLC_TRY(row_view(x, kBwd, "x", vx));
+    if (vx.cols > INT32_MAX / 4) return set_error(TLC_ERR_UNSUPPORTED, "layer_norm_backward: last dim too large");
+    Extent eg, est, ew;
+    TLC_TRY(shaped(grad, kBwd, "grad", x->ndim, x->sizes, false, &eg));
+    TLC_TRY(row_view(grad, kBwd, "grad", vg));
+    int64_t sz[TLC_MAX_DIMS];
+    std::copy(x->sizes, x->sizes + x->ndim, sz);
+    sz[x->ndim - 1] = 2;
+    TLC_TRY(shaped(stats, kBwd, "stats", x->ndim, sz, false, &est));
+    TLC_TRY(row_view(stats, kBwd, "stats", vs));
+    if (weight) TLC_TRY(shaped(weight, kBwd, "weight", 1, &vx.cols, false, &ew));
+    tlc_tensor* outs[3] = {dx, dweight, dbias};
+    const char* names[3] = {"dx", "dweight", "dbias"};
+    Extent eo[3];
+    for (int i = 0; i < 3; ++i) {
+        if (!outs[i]) continue;
+        TLC_TRY(i == 0 ? shaped(dx, kBwd, "dx", x->ndim, x->sizes, true, &eo[0])
+                       : shaped(outs[i], kBwd, names[i], 1, &vx.cols, true, &eo[i]));
+        TLC_TRY(no_overlap(kBwd, names[i], eo[i], "x", vx.ext));
+        TLC_TRY(no_overlap(kBwd, names[i], eo[i], "grad", eg));
+        TLC_TRY(no_overlap(kBwd, names[i], eo[i], "stats", est));
+        TLC_TRY(no_overlap(kBwd, names[i], eo[i], "weight", ew));
+        for (int j = 0; j < i; ++j) TLC_TRY(no_overlap(kBwd, names[i], eo[i], names[j], eo[j]));
+    }
+    if (vx.cols == 0) return TLC_OK;
+    if (vx.rows == 0) {  // a sum over no rows
+        for (int i = 1; i < 3; ++i)
+            if (outs[i] && !accumulate) TLC_TRY(launch_fill_zero(outs[i]->data, vx.cols, s));
+        return TLC_OK;
+    }
+    if (!dx && !dweight && !dbias) return TLC_OK;
+    RowScratch cx(s), cg(s), cs(s), cw(s), cp(s);
+    TLC_TRY(unit_rows(x, vx, cx));
+    TLC_TRY(unit_rows(grad, vg, cg));
+    TLC_TRY(unit_rows(stats, vs, cs));
+    LnBwd p{};
+    TLC_TRY(column_vector(weight, kBwd, "weight", vx.cols, cw, &p.w, &ew));
+    p.g = vg.data;
+    p.x = vx.data;
+    p.stats = vs.data;
+    p.gm = vg.map;
+    p.xm = vx.map;
+    p.sm = vs.map;
+    p.dx = dx ? dx->data : nullptr;
+    p.rows = vx.rows;
+    p.D = (int)vx.cols;
+    p.accumulate = accumulate != 0;
+    const bool sums = dweight || dbias;
+    const bool vec = p.D % 4 == 0 && vx.map.multiple_of(4) && vg.map.multiple_of(4) && aligned_to(p.x, 16) &&
+                     aligned_to(p.g, 16) && aligned_to(p.dx, 16) && aligned_to(p.w, 16);
+    const int threads = bwd_threads(p.D, vec ? 4 : 1);
+    const int sms = sm_count();
+    int parts = 0;
+    if (threads) {
+        const int rpb = threads == 32 ? 8 : 1;
+        const int64_t per_sm = threads == 32 ? 2 : std::max(1, 512 / threads);
+        parts = (int)std::min<int64_t>((p.rows + rpb - 1) / rpb, (int64_t)sms * per_sm);
+        if (sums) {
+            TLC_TRY(scratch_alloc(&cp.p, sizeof(float) * 2 * (size_t)p.D * (size_t)parts, s));
+            p.part = cp.f();
+        }
+        TLC_TRY(vec ? pick_bwd<4>(p, threads, parts, s) : pick_bwd<1>(p, threads, parts, s));
+    } else {
+        if (dx) {
+            ln_bwd_long_kernel<<<(unsigned)std::min<int64_t>(p.rows, INT32_MAX), 1024, 0, s>>>(p);
+            count_launch();
+            TLC_TRY(check_launch(kBwd));
+        }
+        if (sums) {
+            const int64_t cols = ((int64_t)p.D + 255) / 256;
+            const int64_t rows_per = std::max<int64_t>(8, (p.rows * cols + 8 * sms - 1) / (8 * sms));
+            const int64_t chunks = (p.rows + rows_per - 1) / rows_per;
+            parts = (int)chunks;  // at most 8 * sms / cols + 1
+            TLC_TRY(scratch_alloc(&cp.p, sizeof(float) * 2 * (size_t)p.D * (size_t)parts, s));
+            p.part = cp.f();
+            ln_bwd_cols_kernel<<<dim3((unsigned)cols, (unsigned)parts), 256, 0, s>>>(p, rows_per);
+            count_launch();
+            TLC_TRY(check_launch(kBwd));
+        }
+    }
+    if (sums) {
+        const int64_t blocks = (2 * (int64_t)p.D + 31) / 32;
+        ln_bwd_finish_kernel<<<(unsigned)blocks, 256, 0, s>>>(p.part, parts, p.D, dweight ? dweight->data : nullptr,
+                                                             dbias ? dbias->data : nullptr, p.accumulate);
+        count_launch();
+        TLC_TRY(check_launch(kBwd));
+    }
+    return TLC_OK;
+}

@@ -1,0 +1,712 @@
+// Log-probabilities of given tokens under logits [..., V], with the entropy
+// and the most likely alternatives, and the gradient to the logits, fp32.
+//
+//   z_j = scale (x_j - max x),  l = sum e^z_j,  log p_j = z_j - log l
+//   out = log p_t,  H = -sum p_j log p_j = log l - sum e^z_j z_j / l
+//   dx_j = scale (g (1[j = t] - p_j) - h p_j (log p_j + H)),   g, h: the gradients of out and H
+//
+// Everything goes by differences to the row's maximum, so large logits lose
+// nothing; the maximum and log l are what the backward needs (`stats`).
+// One pass over the logits: each thread keeps a running maximum m with
+// l = sum e^(scale (x - m)) and w = sum e^(.) log2 e^(.), rescaled when m
+// grows.  Bound by HBM: 4 bytes a logit forward, 8 backward.
+//
+// A row is read by one block, or by a cluster of blocks when the rows alone
+// would leave SMs idle; short rows by a warp each.
+//
+// The alternatives need no second pass over the row: every thread knows the
+// largest of its own values, so the k-th largest of 64 groups' maxima is a
+// bound that the k largest values all reach, and only the few threads whose
+// maximum reaches it look at their values again.
+//
+// Cases without a distribution: a row of -inf alone has log p = -inf,
+// entropy 0 and no gradient; a NaN or +inf in a row makes its results NaN.
+// Token -1: no token is asked for (log p = 0, no gradient from it); any other
+// token outside [0, V) gives NaN.
+#include <algorithm>
+#include <cmath>
+
+#include "rows.cuh"
+#include "tcgen05.cuh"
+
+namespace tlc {
+namespace {
+
+constexpr const char* kFwd = "token_logprobs";
+constexpr const char* kBwd = "token_logprobs_backward";
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxTop = 32;
+
+// 2^x to 2 ulp, 0 for small x: the probabilities' own rounding is what the sums see.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The larger, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+// Exponents below this give 0; the bound keeps 0 * exponent from being NaN.
+constexpr float kFloor = -160.0f;
+
+// ---- running sums ---------------------------------------------------------------------
+
+// m: maximum (-inf: nothing yet), l = sum 2^y, w = sum 2^y y with y = a (x - m), a = scale log2 e.
+struct Run {
+    float m = -INFINITY, l = 0.0f, w = 0.0f;
+    __device__ __forceinline__ void raise(float to, float a) {
+        if (m == -INFINITY) {
+            m = to;
+            return;
+        }
+        const float y = max_nan((m - to) * a, kFloor);
+        const float c = ex2(y);
+        w = c * fmaf(y, l, w);
+        l *= c;
+        m = to;
+    }
+    __device__ __forceinline__ void merge(const Run& o, float a) {
+        const float to = max_nan(m, o.m);
+        Run q = o;
+        if (m != to) raise(to, a);
+        if (q.m != to) q.raise(to, a);
+        l += q.l;
+        w += q.w;
+        m = to;
+    }
+};
+
+template <int N>
+__device__ __forceinline__ void run_add(Run& r, const float (&v)[N], float a) {
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = max_nan(top, v[i]);
+    if (!(top <= r.m)) r.raise(max_nan(top, r.m), a);  // also when top is NaN
+    const float m = r.m == -INFINITY ? 0.0f : r.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float y = max_nan((v[i] - m) * a, kFloor);
+        const float e = ex2(y);
+        r.l += e;
+        r.w = fmaf(e, y, r.w);
+    }
+}
+
+__device__ __forceinline__ Run warp_run(Run r, float a) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Run q;
+        q.m = __shfl_xor_sync(0xffffffffu, r.m, o);
+        q.l = __shfl_xor_sync(0xffffffffu, r.l, o);
+        q.w = __shfl_xor_sync(0xffffffffu, r.w, o);
+        r.merge(q, a);
+    }
+    return r;
+}
+
+// ---- order of the alternatives --------------------------------------------------------
+
+// Larger value first, NaN before all, then the lower index: one unsigned key.
+__device__ __forceinline__ uint32_t order_of(float v) {
+    if (v != v) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(v + 0.0f);  // -0 as +0
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
+    return ((uint64_t)order_of(v) << 32) | (uint32_t)~index;
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)key; }
+
+struct LpFwd {
+    const float* x;
+    Rows xm;
+    TokenRef tok;
+    int64_t rows;
+    int V;
+    float scale, a;  // a = scale * log2 e
+    float *logp, *entropy, *stats;
+    int top;
+    float* top_logp;
+    void* top_tok;
+    int top_wide;
+};
+
+// What the row's results are, from its sums.
+__device__ __forceinline__ void row_results(const LpFwd& p, int64_t r, const float* x, const Run& s) {
+    const bool none = s.m == -INFINITY;
+    const float log_l = none ? 0.0f : logf(s.l);
+    if (p.stats) {
+        p.stats[2 * r] = s.m;
+        p.stats[2 * r + 1] = log_l;
+    }
+    if (p.entropy) p.entropy[r] = none ? 0.0f : fmaxf(log_l - kLn2 * (s.w / s.l), 0.0f) + (s.l != s.l ? s.l : 0.0f);
+    if (p.logp) {
+        const int64_t t = p.tok.get(r);
+        float lp = 0.0f;
+        if (t != -1) {
+            if (t < 0 || t >= p.V)
+                lp = __int_as_float(0x7fc00000);
+            else
+                lp = none ? -INFINITY : (x[t] - s.m) * p.scale - log_l;
+        }
+        p.logp[r] = lp;
+    }
+}
+
+__device__ __forceinline__ void top_result(const LpFwd& p, int64_t r, const float* x, int i, uint64_t key, float m,
+                                           float log_l) {
+    const uint32_t j = index_of(key);
+    p.top_logp[r * p.top + i] = m == -INFINITY ? -INFINITY : (x[j] - m) * p.scale - log_l;
+    if (p.top_wide)
+        static_cast<int64_t*>(p.top_tok)[r * p.top + i] = j;
+    else
+        static_cast<int32_t*>(p.top_tok)[r * p.top + i] = (int32_t)j;
+}
+
+// ---- a row for a warp -------------------------------------------------------------------
+
+// V <= 32 * VPT, the values in registers (element 32 i + lane).
+template <int VPT>
+__global__ void __launch_bounds__(256) lp_warp_kernel(LpFwd p) {
+    const int lane = threadIdx.x & 31;
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < p.rows; r += (int64_t)gridDim.x * 8) {
+        const float* x = p.x + p.xm.offset(r);
+        float v[VPT];
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) v[i] = 32 * i + lane < p.V ? __ldcs(x + 32 * i + lane) : -INFINITY;
+        Run s;
+        run_add(s, v, p.a);
+        s = warp_run(s, p.a);
+        // a lane without values of its own still counted -inf: nothing
+        if (lane == 0) row_results(p, r, x, s);
+        if (p.top) {
+            const float log_l = s.m == -INFINITY ? 0.0f : logf(s.l);
+            uint64_t last = ~0ull;  // the key picked before
+            for (int i = 0; i < p.top; ++i) {
+                uint64_t best = 0;
+#pragma unroll
+                for (int q = 0; q < VPT; ++q) {
+                    const uint32_t j = 32 * q + lane;
+                    if (j < (uint32_t)p.V) {
+                        const uint64_t k = key_of(v[q], j);
+                        if (k < last && k > best) best = k;
+                    }
+                }
+                const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+                const uint32_t lo =
+                    __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+                last = ((uint64_t)hi << 32) | lo;
+                if (lane == 0) top_result(p, r, x, i, last, s.m, log_l);
+            }
+        }
+    }
+}
+
+// ---- a row for a block or a cluster of blocks ----------------------------------------------
+
+constexpr int CAP = 512;  // candidates for the alternatives that a block keeps
+
+template <int T>
+struct LpSmem {
+    float m[T / 32], l[T / 32], w[T / 32];
+    float row_m, row_l, row_w;         // the block's sums, read by the cluster's first block
+    uint32_t group[64];
+    uint32_t bound;
+    int threads, found;
+    uint16_t look[T];                  // threads whose values reach the bound
+    uint64_t cand[CAP];
+    uint64_t best[kMaxTop];            // the block's alternatives, in order
+    uint64_t all[16 * kMaxTop];        // the cluster's, in its first block
+    uint32_t hist[256];
+    int bin, need;
+};
+
+// A block's part of a row: the first `head` values singly up to a 16-byte
+// boundary, then `vecs` float4, then `tail` values.
+struct Part {
+    const float* x;  // the part's first value
+    int first, n;    // its index in the row, and how many
+    int head, vecs, tail;
+    __device__ __forceinline__ Part(const float* row, int lo, int hi) {
+        x = row + lo;
+        first = lo;
+        n = hi - lo;
+        head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) >> 2);
+        vecs = (n - head) >> 2;
+        tail = n - head - 4 * vecs;
+    }
+    __device__ __forceinline__ float4 vec(int i) const {
+        return __ldcs(reinterpret_cast<const float4*>(x + head) + i);
+    }
+    // the single value of thread t < 6, if it has one: its position in the part, or -1
+    __device__ __forceinline__ int single(int t) const {
+        if (t < 3) return t < head ? t : -1;
+        if (t < 6) return t - 3 < tail ? head + 4 * vecs + t - 3 : -1;
+        return -1;
+    }
+};
+
+// The part's `k` largest keys in order, into sm.best (k <= part.n values; the
+// rest of sm.best is 0).  top: the largest value of this thread (-inf: none).
+template <int T>
+__device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int G = T / 64;  // neighbouring lanes a group
+    uint32_t g = order_of(top);
+#pragma unroll
+    for (int o = 1; o < G; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (tid % G == 0) sm.group[tid / G] = g;
+    if (tid == 0) sm.threads = sm.found = 0;
+    if (tid < kMaxTop) sm.best[tid] = 0;
+    __syncthreads();
+    if (tid < 64) {  // the k-th largest of the groups' maxima
+        const uint32_t v = sm.group[tid];
+        int above = 0;
+        for (int j = 0; j < 64; ++j) {
+            const uint32_t o = sm.group[j];
+            above += o > v || (o == v && j < tid);
+        }
+        if (above == k - 1) sm.bound = v;
+    }
+    __syncthreads();
+    const uint32_t bound = sm.bound;
+    if (order_of(top) >= bound) sm.look[atomicAdd(&sm.threads, 1)] = (uint16_t)tid;
+    __syncthreads();
+    const int threads = sm.threads;
+    auto take = [&](float v, int at) {
+        if (order_of(v) >= bound) {
+            const int c = atomicAdd(&sm.found, 1);
+            if (c < CAP) sm.cand[c] = key_of(v, (uint32_t)(part.first + at));
+        }
+    };
+    for (int q = warp; q < threads; q += T / 32) {
+        const int t = sm.look[q];
+        for (int i = t + T * lane; i < part.vecs; i += T * 32) {
+            const float4 f = part.vec(i);
+            const int at = part.head + 4 * i;
+            take(f.x, at);
+            take(f.y, at + 1);
+            take(f.z, at + 2);
+            take(f.w, at + 3);
+        }
+        if (lane == 0) {
+            const int at = part.single(t);
+            if (at >= 0) take(part.x[at], at);
+        }
+    }
+    __syncthreads();
+    int found = sm.found;
+    if (found > CAP) {
+        // Too many values reach the bound (equal logits, or few that are not
+        // masked): find the k-th largest key digit by digit, reading the part
+        // once for each of the 8 digits, then take the k keys from it up.
+        uint64_t prefix = 0;
+        if (tid == 0) sm.need = k;
+        for (int shift = 56; shift >= 0; shift -= 8) {
+            for (int b = tid; b < 256; b += T) sm.hist[b] = 0;
+            __syncthreads();
+            for (int i0 = 0; i0 < part.n; i0 += T) {
+                const int i = i0 + tid;
+                const uint64_t key = i < part.n ? key_of(part.x[i], (uint32_t)(part.first + i)) : 0;
+                const bool in = i < part.n && (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
+                const uint32_t bin = (uint32_t)(key >> shift) & 255u;
+                const uint32_t act = __ballot_sync(0xffffffffu, in);
+                if (act) {
+                    // equal digits are the rule here: one add for the lanes that share the first one's
+                    const uint32_t b0 = __shfl_sync(0xffffffffu, bin, __ffs(act) - 1);
+                    const uint32_t same = __ballot_sync(0xffffffffu, in && bin == b0);
+                    if (lane == __ffs(act) - 1) atomicAdd(&sm.hist[b0], (uint32_t)__popc(same));
+                    if (in && bin != b0) atomicAdd(&sm.hist[bin], 1u);
+                }
+            }
+            __syncthreads();
+            if (tid == 0) {
+                int need = sm.need, b = 255;
+                while (b > 0 && (int)sm.hist[b] < need) need -= (int)sm.hist[b--];
+                sm.bin = b;
+                sm.need = need;
+            }
+            __syncthreads();
+            prefix |= (uint64_t)(uint32_t)sm.bin << shift;
+            __syncthreads();
+        }
+        if (tid == 0) sm.found = 0;
+        __syncthreads();
+        for (int i = tid; i < part.n; i += T) {
+            const uint64_t key = key_of(part.x[i], (uint32_t)(part.first + i));
+            if (key >= prefix) sm.cand[min(atomicAdd(&sm.found, 1), CAP - 1)] = key;
+        }
+        __syncthreads();
+        found = min(sm.found, CAP);
+    }
+    for (int c = tid; c < found; c += T) {
+        const uint64_t key = sm.cand[c];
+        int above = 0;
+        for (int o = 0; o < found; ++o) above += sm.cand[o] > key;
+        if (above < k) sm.best[above] = key;
+    }
+    __syncthreads();
+}
+
+// C blocks a row (1, or the cluster's size), T threads a block.
+template <int T>
+__global__ void __launch_bounds__(T) lp_row_kernel(LpFwd p, int C) {
+    __shared__ LpSmem<T> sm;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = C > 1 ? (int)cluster_ctarank() : 0;
+    const int64_t r = blockIdx.x / C;
+    const float* x = p.x + p.xm.offset(r);
+    const int per = ((p.V + C - 1) / C + 31) & ~31;
+    const int lo = (int)min((int64_t)p.V, (int64_t)rank * per), hi = (int)min((int64_t)p.V, (int64_t)lo + per);
+    const Part part(x, lo, hi);
+    Run s;
+    constexpr int U = 4;
+    int i = tid;
+    for (; i + (U - 1) * T < part.vecs; i += U * T) {
+        float v[4 * U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float4 f = part.vec(i + u * T);
+            v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
+        }
+        run_add(s, v, p.a);
+    }
+    for (; i < part.vecs; i += T) {
+        const float4 f = part.vec(i);
+        const float v[4] = {f.x, f.y, f.z, f.w};
+        run_add(s, v, p.a);
+    }
+    if (const int at = part.single(tid); at >= 0) {
+        const float v[1] = {part.x[at]};
+        run_add(s, v, p.a);
+    }
+    const float top = s.m;
+    s = warp_run(s, p.a);
+    if (lane == 0) sm.m[warp] = s.m, sm.l[warp] = s.l, sm.w[warp] = s.w;
+    __syncthreads();
+    if (warp == 0) {
+        Run q;
+        if (lane < T / 32) q.m = sm.m[lane], q.l = sm.l[lane], q.w = sm.w[lane];
+        q = warp_run(q, p.a);
+        if (lane == 0) sm.row_m = q.m, sm.row_l = q.l, sm.row_w = q.w;
+    }
+    const int k = min(p.top, part.n);
+    if (p.top > 0 && k > 0) part_top(sm, part, k, top);
+    else if (p.top > 0 && tid < kMaxTop) sm.best[tid] = 0;
+    __syncthreads();
+    if (C == 1) {
+        if (tid == 0) {
+            Run q;
+            q.m = sm.row_m, q.l = sm.row_l, q.w = sm.row_w;
+            row_results(p, r, x, q);
+        }
+        if (tid < p.top) {
+            const float log_l = sm.row_m == -INFINITY ? 0.0f : logf(sm.row_l);
+            top_result(p, r, x, tid, sm.best[tid], sm.row_m, log_l);
+        }
+        return;
+    }
+    cluster_sync();
+    if (rank == 0) {
+        if (warp == 0) {
+            Run q;
+            if (lane < C) {
+                auto get = [&](const float* f) {
+                    float v;
+                    const uint32_t at = mapa(static_cast<uint32_t>(__cvta_generic_to_shared(f)), (uint32_t)lane);
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+                    return v;
+                };
+                q.m = get(&sm.row_m), q.l = get(&sm.row_l), q.w = get(&sm.row_w);
+            }
+            q = warp_run(q, p.a);
+            if (lane == 0) {
+                row_results(p, r, x, q);
+                sm.m[0] = q.m, sm.l[0] = q.l;
+            }
+        }
+        for (int c = tid; c < C * p.top; c += T) {
+            const int from = c / p.top;
+            const uint32_t at =
+                mapa(static_cast<uint32_t>(__cvta_generic_to_shared(&sm.best[c - from * p.top])), (uint32_t)from);
+            asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(sm.all[c]) : "r"(at) : "memory");
+        }
+        __syncthreads();
+        const float log_l = sm.m[0] == -INFINITY ? 0.0f : logf(sm.l[0]);
+        for (int c = tid; c < C * p.top; c += T) {
+            const uint64_t key = sm.all[c];
+            if (key == 0) continue;  // a block with fewer values
+            int above = 0;
+            for (int o = 0; o < C * p.top; ++o) above += sm.all[o] > key;
+            if (above < p.top) top_result(p, r, x, above, key, sm.m[0], log_l);
+        }
+    }
+    cluster_sync();  // the first block has read the others' shared memory
+}
+
+// ---- the gradient ---------------------------------------------------------------------------
+
+struct LpBwd {
+    const float *x, *stats, *entropy, *g, *h;
+    Rows xm, sm, em, gm, hm;
+    TokenRef tok;
+    float* dx;  // may be x itself: each value is read and written by one thread
+    int64_t rows;
+    int V;
+    float scale;
+};
+
+struct RowGrad {
+    float m, log_l, H, g, h, scale;
+    int64_t t;
+    bool none;
+    __device__ __forceinline__ RowGrad(const LpBwd& p, int64_t r) {
+        const float* st = p.stats + p.sm.offset(r);
+        m = st[0], log_l = st[1];
+        t = p.tok.get(r);
+        g = p.g && t != -1 ? p.g[p.gm.offset(r)] : 0.0f;
+        if (p.g && (t < -1 || t >= p.V)) g = __int_as_float(0x7fc00000);
+        h = p.h ? p.h[p.hm.offset(r)] : 0.0f;
+        H = p.h ? p.entropy[p.em.offset(r)] : 0.0f;
+        none = m == -INFINITY;
+        scale = p.scale;
+    }
+    __device__ __forceinline__ float at(float x, int64_t j) const {
+        if (none) return 0.0f;
+        const float lp = max_nan(fmaf(x - m, scale, -log_l), kFloor);
+        const float pr = expf(lp);  // to 1 ulp: the SMs have time for it beside 8 bytes a value
+        // g (1[j = t] - p) - h p (log p + H)
+        float d = -pr * fmaf(h, lp + H, g);
+        if (j == t) d += g;
+        return d * scale;
+    }
+};
+
+// 256 threads for a run of BW values of one row.
+constexpr int BW = 8192;
+template <bool VEC>
+__global__ void __launch_bounds__(256) lp_bwd_kernel(LpBwd p, int pieces) {
+    const int64_t r = blockIdx.x / pieces;
+    const int lo = (int)(blockIdx.x - r * pieces) * BW, hi = min(p.V, lo + BW);
+    const float* x = p.x + p.xm.offset(r);
+    float* dx = p.dx + r * p.V;
+    const RowGrad q(p, r);
+    if constexpr (VEC) {
+        const Part part(x, lo, hi);
+        float* d = dx + lo;
+        for (int i = threadIdx.x; i < part.vecs; i += 256) {
+            const float4 f = *(reinterpret_cast<const float4*>(part.x + part.head) + i);
+            const int64_t j = lo + part.head + 4 * i;
+            float4 y;
+            y.x = q.at(f.x, j), y.y = q.at(f.y, j + 1), y.z = q.at(f.z, j + 2), y.w = q.at(f.w, j + 3);
+            *(reinterpret_cast<float4*>(d + part.head) + i) = y;
+        }
+        if (const int at = part.single(threadIdx.x); at >= 0) d[at] = q.at(part.x[at], lo + at);
+    } else {
+        for (int j = lo + threadIdx.x; j < hi; j += 256) dx[j] = q.at(x[j], j);
+    }
+}
+
+// A warp a row.
+__global__ void __launch_bounds__(256) lp_bwd_warp_kernel(LpBwd p) {
+    const int lane = threadIdx.x & 31;
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < p.rows; r += (int64_t)gridDim.x * 8) {
+        const float* x = p.x + p.xm.offset(r);
+        float* dx = p.dx + r * p.V;
+        const RowGrad q(p, r);
+        for (int j = lane; j < p.V; j += 32) dx[j] = q.at(x[j], j);
+    }
+}
+
+template <int VPT>
+int launch_warp(const LpFwd& p, cudaStream_t s) {
+    const unsigned grid = (unsigned)std::min<int64_t>((p.rows + 7) / 8, INT32_MAX);
+    lp_warp_kernel<VPT><<<grid, 256, 0, s>>>(p);
+    count_launch();
+    return check_launch(kFwd);
+}
+
+template <int T>
+int launch_row(const LpFwd& p, int C, cudaStream_t s) {
+    if (p.rows * C > INT32_MAX) return set_error(TLC_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(p.rows * C));
+    cfg.blockDim = dim3(T);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = C > 1 ? 1 : 0;
+    TLC_CUDA_TRY(cudaLaunchKernelEx(&cfg, lp_row_kernel<T>, p, C));
+    count_launch();
+    return check_launch(kFwd);
+}
+
+int check_scale(float scale, const char* op) {
+    if (std::isfinite(scale) && scale > 0.0f) return TLC_OK;
+    return set_error(TLC_ERR_INVALID_ARGUMENT, std::string(op) + ": scale must be positive and finite");
+}
+
+// tokens (and others) have the shape of the logits without their last dim
+int same_lead(const tlc_tensor* logits, int nd, const int64_t* sizes, const char* op, const char* name) {
+    bool same = nd == logits->ndim - 1;
+    for (int i = 0; same && i < nd; ++i) same = sizes[i] == logits->sizes[i];
+    if (same) return TLC_OK;
+    return set_error(TLC_ERR_INVALID_ARGUMENT, std::string(op) + ": " + name + ": wrong shape");
+}
+
+}  // namespace
+}  // namespace tlc
+
+using namespace tlc;
+
+extern "C" int tlc_token_logprobs(const tlc_tensor* logits, const tlc_index* tokens, float scale,
+                                  tlc_tensor* logprobs, tlc_tensor* entropy, tlc_tensor* stats, int top,
+                                  tlc_tensor* top_logprobs, tlc_index* top_tokens, void* stream) {
+    clear_error();
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    RowView vx;
+    LpFwd p{};
+    int64_t n = 0, sz[TLC_MAX_DIMS];
+    Extent et, eo[5];
+    TLC_TRY(row_view(logits, kFwd, "logits", vx));
+    TLC_TRY(check_scale(scale, kFwd));
+    if (vx.cols > (1 << 30)) return set_error(TLC_ERR_UNSUPPORTED, "token_logprobs: vocabulary too large");
+    const int nd = logits->ndim - 1;
+    if (logprobs) {
+        TLC_TRY(index_view(tokens, kFwd, "tokens", p.tok, &n, &et));
+        TLC_TRY(same_lead(logits, tokens->ndim, tokens->sizes, kFwd, "tokens"));
+    }
+    if (top < 0 || top > vx.cols)
+        return set_error(TLC_ERR_INVALID_ARGUMENT, "token_logprobs: top must be 0 to the vocabulary's size");
+    if (top > kMaxTop)
+        return set_error(TLC_ERR_UNSUPPORTED, "token_logprobs: top is at most " + std::to_string(kMaxTop));
+    if (vx.rows > 0 && vx.cols == 0)
+        return set_error(TLC_ERR_INVALID_ARGUMENT, "token_logprobs: rows without logits");
+    const char* names[5] = {"logprobs", "entropy", "stats", "top_logprobs", "top_tokens"};
+    if (logprobs) TLC_TRY(shaped(logprobs, kFwd, names[0], nd, logits->sizes, true, &eo[0]));
+    if (entropy) TLC_TRY(shaped(entropy, kFwd, names[1], nd, logits->sizes, true, &eo[1]));
+    std::copy(logits->sizes, logits->sizes + nd, sz);
+    sz[nd] = 2;
+    if (stats) TLC_TRY(shaped(stats, kFwd, names[2], nd + 1, sz, true, &eo[2]));
+    if (top) {
+        sz[nd] = top;
+        TLC_TRY(shaped(top_logprobs, kFwd, names[3], nd + 1, sz, true, &eo[3]));
+        TokenRef ref;
+        int64_t cnt;
+        TLC_TRY(index_view(top_tokens, kFwd, names[4], ref, &cnt, &eo[4]));
+        bool same = top_tokens->ndim == nd + 1;
+        for (int i = 0; same && i <= nd; ++i) same = top_tokens->sizes[i] == sz[i];
+        if (!same) return set_error(TLC_ERR_INVALID_ARGUMENT, "token_logprobs: top_tokens: wrong shape");
+        if (!dense_strides(nd + 1, top_tokens->sizes, top_tokens->strides))
+            return set_error(TLC_ERR_INVALID_ARGUMENT, "token_logprobs: top_tokens must be contiguous");
+    }
+    for (int i = 0; i < 5; ++i) {
+        TLC_TRY(no_overlap(kFwd, names[i], eo[i], "logits", vx.ext));
+        TLC_TRY(no_overlap(kFwd, names[i], eo[i], "tokens", et));
+        for (int j = 0; j < i; ++j) TLC_TRY(no_overlap(kFwd, names[i], eo[i], names[j], eo[j]));
+    }
+    if (vx.rows == 0) return TLC_OK;
+    RowScratch cx(s);
+    TLC_TRY(unit_rows(logits, vx, cx));
+    p.x = vx.data;
+    p.xm = vx.map;
+    p.rows = vx.rows;
+    p.V = (int)vx.cols;
+    p.scale = scale;
+    p.a = scale * kLog2e;
+    p.logp = logprobs ? logprobs->data : nullptr;
+    p.entropy = entropy ? entropy->data : nullptr;
+    p.stats = stats ? stats->data : nullptr;
+    p.top = top;
+    if (top) {
+        p.top_logp = top_logprobs->data;
+        p.top_tok = top_tokens->data;
+        p.top_wide = top_tokens->bits == 64;
+    }
+    if (p.V <= 128) return launch_warp<4>(p, s);
+    if (p.V <= 512) return launch_warp<16>(p, s);
+    if (p.V <= 1024) return launch_warp<32>(p, s);
+    int C = 1;
+    while (C < 8 && p.rows * C * 2 <= 148 && p.V / (2 * C) >= 2048) C *= 2;
+    return C > 1 ? launch_row<512>(p, C, s) : launch_row<256>(p, C, s);
+}
+
+extern "C" int tlc_token_logprobs_backward(const tlc_tensor* logits, const tlc_index* tokens,
+                                           const tlc_tensor* stats, const tlc_tensor* entropy,
+                                           const tlc_tensor* grad_logprobs, const tlc_tensor* grad_entropy,
+                                           float scale, tlc_tensor* dlogits, void* stream) {
+    clear_error();
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    RowView vx, vs;
+    LpBwd p{};
+    int64_t n = 0, sz[TLC_MAX_DIMS];
+    Extent et, es, ee, eg, eh, ed;
+    TLC_TRY(row_view(logits, kBwd, "logits", vx));
+    TLC_TRY(check_scale(scale, kBwd));
+    if (vx.cols > (1 << 30)) return set_error(TLC_ERR_UNSUPPORTED, "token_logprobs_backward: vocabulary too large");
+    const int nd = logits->ndim - 1;
+    TLC_TRY(index_view(tokens, kBwd, "tokens", p.tok, &n, &et));
+    TLC_TRY(same_lead(logits, tokens->ndim, tokens->sizes, kBwd, "tokens"));
+    std::copy(logits->sizes, logits->sizes + nd, sz);
+    sz[nd] = 2;
+    TLC_TRY(shaped(stats, kBwd, "stats", nd + 1, sz, false, &es));
+    TLC_TRY(row_view(stats, kBwd, "stats", vs));
+    if (grad_logprobs) {
+        TLC_TRY(shaped(grad_logprobs, kBwd, "grad_logprobs", nd, logits->sizes, false, &eg));
+        p.g = grad_logprobs->data;
+        p.gm = merge_rows(nd, grad_logprobs->sizes, grad_logprobs->strides);
+    }
+    if (grad_entropy) {
+        TLC_TRY(shaped(grad_entropy, kBwd, "grad_entropy", nd, logits->sizes, false, &eh));
+        TLC_TRY(shaped(entropy, kBwd, "entropy", nd, logits->sizes, false, &ee));
+        p.h = grad_entropy->data;
+        p.hm = merge_rows(nd, grad_entropy->sizes, grad_entropy->strides);
+        p.entropy = entropy->data;
+        p.em = merge_rows(nd, entropy->sizes, entropy->strides);
+    }
+    TLC_TRY(shaped(dlogits, kBwd, "dlogits", logits->ndim, logits->sizes, true, &ed));
+    const bool in_place = dlogits->data == logits->data && dense_strides(logits->ndim, logits->sizes, logits->strides);
+    if (!in_place) TLC_TRY(no_overlap(kBwd, "dlogits", ed, "logits", vx.ext));
+    TLC_TRY(no_overlap(kBwd, "dlogits", ed, "tokens", et));
+    TLC_TRY(no_overlap(kBwd, "dlogits", ed, "stats", es));
+    TLC_TRY(no_overlap(kBwd, "dlogits", ed, "entropy", ee));
+    TLC_TRY(no_overlap(kBwd, "dlogits", ed, "grad_logprobs", eg));
+    TLC_TRY(no_overlap(kBwd, "dlogits", ed, "grad_entropy", eh));
+    if (vx.numel == 0) return TLC_OK;
+    RowScratch cx(s), cs(s);
+    TLC_TRY(unit_rows(logits, vx, cx));
+    TLC_TRY(unit_rows(stats, vs, cs));
+    p.x = vx.data;
+    p.xm = vx.map;
+    p.stats = vs.data;
+    p.sm = vs.map;
+    p.dx = dlogits->data;
+    p.rows = vx.rows;
+    p.V = (int)vx.cols;
+    p.scale = scale;
+    if (p.V <= 1024) {
+        lp_bwd_warp_kernel<<<(unsigned)std::min<int64_t>((p.rows + 7) / 8, INT32_MAX), 256, 0, s>>>(p);
+    } else {
+        const int pieces = (p.V + BW - 1) / BW;
+        if (p.rows * pieces > INT32_MAX)
+            return set_error(TLC_ERR_UNSUPPORTED, "token_logprobs_backward: too many rows");
+        // float4 where each row of x and dx starts at the same place within 16 bytes
+        const bool vec = (reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.dx)) % 16 == 0 &&
+                         (p.rows == 1 || (p.xm.nd == 1 && (p.xm.st[0] - p.V) % 4 == 0) ||
+                          (p.V % 4 == 0 && p.xm.multiple_of(4)));
+        const unsigned grid = (unsigned)(p.rows * pieces);
+        if (vec)
+            lp_bwd_kernel<true><<<grid, 256, 0, s>>>(p, pieces);
+        else
+            lp_bwd_kernel<false><<<grid, 256, 0, s>>>(p, pieces);
+    }
+    count_launch();
+    return check_launch(kBwd);
+}

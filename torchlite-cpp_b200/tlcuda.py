@@ -51,9 +51,15 @@ class GemmDesc(ctypes.Structure):
                 ("c_bstride", ctypes.c_int64 * 3)]
 
 
+class Index(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("ndim", ctypes.c_int32), ("bits", ctypes.c_int32),
+                ("sizes", ctypes.c_int64 * MAX_DIMS), ("strides", ctypes.c_int64 * MAX_DIMS)]
+
+
 # Every symbol include/tlc.h declares, with its ctypes signature.
 _P = ctypes.POINTER
 _T = _P(Tensor)
+_I = _P(Index)
 _v, _i, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 SIGNATURES = {
     "tlc_version": ([], _i),
@@ -97,6 +103,12 @@ SIGNATURES = {
     "tlc_flash_attention": ([_T, _T, _T, ctypes.c_float, _T, _T, _i, _v], _i),
     "tlc_flash_attention_backward": ([_T, _T, _T, _T, _T, _T, ctypes.c_float, _T, _T, _T, _i, _v],
                                      _i),
+    "tlc_layer_norm": ([_T, _T, _T, ctypes.c_float, _T, _T, _v], _i),
+    "tlc_layer_norm_backward": ([_T, _T, _T, _T, _T, _T, _T, _i, _v], _i),
+    "tlc_embedding": ([_T, _I, ctypes.c_float, _T, _v], _i),
+    "tlc_embedding_backward": ([_T, _I, ctypes.c_float, _T, _i, _v], _i),
+    "tlc_token_logprobs": ([_T, _I, ctypes.c_float, _T, _T, _T, _i, _T, _I, _v], _i),
+    "tlc_token_logprobs_backward": ([_T, _I, _T, _T, _T, _T, ctypes.c_float, _T, _v], _i),
     "tlc_load_tlmd": ([ctypes.c_char_p, ctypes.c_int32, _T, _v], _i),
     "tlc_save_tlmd": ([ctypes.c_char_p, ctypes.c_int32, _T, _v], _i),
     "tlc_shard_range": ([_i64, _i, _i, _P(_i64), _P(_i64)], _i),
@@ -420,6 +432,160 @@ def flash_attention_backward(grad, q, k, v, out, lse, sm_scale, mode="exact", dq
                                               *[ctypes.byref(x) for x in vd], mode_id(mode),
                                               _stream_ptr(stream)))
     return dq, dk, dv
+
+
+# ---- token models: layer norm, embedding, token log-probabilities ------------------------
+# These check what the C ABI cannot see (types, and that every tensor is on the
+# current device) and raise ValueError; shapes and strides are checked there.
+
+_SHAPE = ctypes.c_int64 * MAX_DIMS
+
+
+def _dev_view(t, name):
+    """tlc_tensor of a float32 CUDA tensor on the current device (None stays None)."""
+    import torch
+    if t is None:
+        return None
+    if t.dtype != torch.float32:
+        raise ValueError(f"{name}: libtl_cuda computes in float32, not {t.dtype}")
+    _on_current(t, name)
+    return Tensor(t.data_ptr(), t.dim(), _SHAPE(*t.shape), _SHAPE(*t.stride()))
+
+
+def _index_view(t, name):
+    """tlc_index of an int32 or int64 CUDA tensor on the current device."""
+    import torch
+    if t is None:
+        return None
+    if t.dtype is not torch.int64 and t.dtype is not torch.int32:
+        raise ValueError(f"{name}: int32 or int64, not {t.dtype}")
+    _on_current(t, name)
+    return Index(t.data_ptr(), t.dim(), 64 if t.dtype is torch.int64 else 32, _SHAPE(*t.shape),
+                 _SHAPE(*t.stride()))
+
+
+def _on_current(t, name):
+    import torch
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+    if t.dim() > MAX_DIMS:
+        raise ValueError(f"{name}: at most {MAX_DIMS} dims")
+
+
+def _new(like, shape, dtype=None):
+    import torch
+    return torch.empty(shape, dtype=dtype or torch.float32, device=like.device)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None, stats=None, need_stats=True,
+               stream=None):
+    """Layer norm over the last dim: returns (out, stats), stats [..., 2] = (mean, rstd) of
+    each row, what the backward needs (None with need_stats=False)."""
+    if x.dim() == 0:
+        raise ValueError("layer_norm: x must be at least 1-D")
+    if out is None:
+        out = _new(x, x.shape)
+    if stats is None and need_stats:
+        stats = _new(x, (*x.shape[:-1], 2))
+    _check(lib().tlc_layer_norm(_dev_view(x, "x"), _dev_view(weight, "weight"),
+                                _dev_view(bias, "bias"), eps, _dev_view(out, "out"),
+                                _dev_view(stats, "stats"), _stream_ptr(stream)))
+    return out, stats
+
+
+def layer_norm_backward(grad, x, stats, weight=None, need=(True, True, True), dx=None,
+                        dweight=None, dbias=None, accumulate=False, stream=None):
+    """Gradients of layer_norm: (dx, dweight, dbias), None where not requested.  With
+    accumulate, given outputs receive their old values plus the gradient."""
+    if x.dim() == 0:
+        raise ValueError("layer_norm_backward: x must be at least 1-D")
+    outs = []
+    for want, t, shape in zip(need, (dx, dweight, dbias), (x.shape, x.shape[-1:], x.shape[-1:])):
+        if want and t is None:
+            if accumulate:
+                raise ValueError("layer_norm_backward: accumulate needs the outputs it adds to")
+            t = _new(x, shape)
+        outs.append(t if want else None)
+    _check(lib().tlc_layer_norm_backward(
+        _dev_view(grad, "grad"), _dev_view(x, "x"), _dev_view(stats, "stats"),
+        _dev_view(weight, "weight"), _dev_view(outs[0], "dx"), _dev_view(outs[1], "dweight"),
+        _dev_view(outs[2], "dbias"), int(accumulate), _stream_ptr(stream)))
+    return tuple(outs)
+
+
+def embedding(weight, tokens, scale=1.0, out=None, stream=None):
+    """out[i] = scale * weight[tokens[i]]; token -1 (padding) gives zeros, any other token
+    outside the table a row of NaN."""
+    if weight.dim() != 2:
+        raise ValueError("embedding: weight must be 2-D")
+    if out is None:
+        out = _new(weight, (*tokens.shape, weight.shape[1]))
+    _check(lib().tlc_embedding(_dev_view(weight, "weight"), _index_view(tokens, "tokens"), scale,
+                               _dev_view(out, "out"), _stream_ptr(stream)))
+    return out
+
+
+def embedding_backward(grad, tokens, rows=None, scale=1.0, dweight=None, accumulate=False,
+                       stream=None):
+    """The table's gradient [rows, D]: sums of grad over the positions of each token, times
+    scale.  With accumulate they are added to `dweight`."""
+    if grad.dim() == 0:
+        raise ValueError("embedding_backward: grad must be at least 1-D")
+    if dweight is None:
+        if accumulate:
+            raise ValueError("embedding_backward: accumulate needs the dweight it adds to")
+        if rows is None:
+            raise ValueError("embedding_backward: rows (the table's length) or dweight is needed")
+        dweight = _new(grad, (rows, grad.shape[-1]))
+    elif rows is not None and rows != dweight.shape[0]:
+        raise ValueError("embedding_backward: dweight has another number of rows")
+    _check(lib().tlc_embedding_backward(_dev_view(grad, "grad"), _index_view(tokens, "tokens"),
+                                        scale, _dev_view(dweight, "dweight"), int(accumulate),
+                                        _stream_ptr(stream)))
+    return dweight
+
+
+def token_logprobs(logits, tokens=None, scale=1.0, top=0, need_entropy=True, need_stats=True,
+                   stream=None):
+    """Of p = softmax(scale * logits) over the last dim: (logprobs, entropy, stats,
+    top_logprobs, top_tokens), None where not requested.  logprobs: log p of the given tokens
+    (0 for token -1); stats: what token_logprobs_backward needs; top_*: the `top` (at most 32)
+    most likely tokens in order, of the type of `tokens` (int64 without tokens)."""
+    import torch
+    if logits.dim() == 0:
+        raise ValueError("token_logprobs: logits must be at least 1-D")
+    lead = logits.shape[:-1]
+    logp = _new(logits, lead) if tokens is not None else None
+    entropy = _new(logits, lead) if need_entropy else None
+    stats = _new(logits, (*lead, 2)) if need_stats else None
+    top_logp = top_tokens = None
+    if top:
+        top_logp = _new(logits, (*lead, top))
+        top_tokens = _new(logits, (*lead, top), tokens.dtype if tokens is not None else torch.int64)
+    _check(lib().tlc_token_logprobs(
+        _dev_view(logits, "logits"), _index_view(tokens, "tokens"), scale,
+        _dev_view(logp, "logprobs"), _dev_view(entropy, "entropy"), _dev_view(stats, "stats"), top,
+        _dev_view(top_logp, "top_logprobs"), _index_view(top_tokens, "top_tokens"),
+        _stream_ptr(stream)))
+    return logp, entropy, stats, top_logp, top_tokens
+
+
+def token_logprobs_backward(logits, tokens, stats, grad_logprobs=None, grad_entropy=None,
+                            entropy=None, scale=1.0, out=None, stream=None):
+    """The gradient to the logits from those of logprobs and entropy (with grad_entropy the
+    forward's entropy is needed).  `out` may be the (contiguous) logits themselves."""
+    if logits.dim() == 0:
+        raise ValueError("token_logprobs_backward: logits must be at least 1-D")
+    if grad_entropy is not None and entropy is None:
+        raise ValueError("token_logprobs_backward: grad_entropy needs the forward's entropy")
+    if out is None:
+        out = _new(logits, logits.shape)
+    _check(lib().tlc_token_logprobs_backward(
+        _dev_view(logits, "logits"), _index_view(tokens, "tokens"), _dev_view(stats, "stats"),
+        _dev_view(entropy, "entropy"), _dev_view(grad_logprobs, "grad_logprobs"),
+        _dev_view(grad_entropy, "grad_entropy"), scale, _dev_view(out, "out"),
+        _stream_ptr(stream)))
+    return out
 
 
 def _views(tensors):
