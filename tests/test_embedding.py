@@ -275,4 +275,4 @@ def test_binding_refusals():
     with pytest.raises(ValueError, match="another number of rows"):
         tlcuda.embedding_backward(w, t, 5, dweight=w)
     with pytest.raises(ValueError, match="int32 or int64"):
-        tlcuda._index_view(w, "tokens")
+        tlcuda.embedding(w, w)

@@ -81,19 +81,22 @@ struct Extent {
     bool overlaps(const Extent& o) const { return lo < hi && o.lo < o.hi && lo < o.hi && o.lo < hi; }
 };
 
+// A refusal, and its message "op: name<what>" (built only then: small calls are bound by the host).
+inline int bad(const char* op, const char* name, const char* what) {
+    return set_error(TLC_ERR_INVALID_ARGUMENT, std::string(op) + ": " + name + what);
+}
+
 // Checks of one view (`bytes` an element): rank 1..8 (or 0), sizes and strides
 // not negative, a size that fits, an address that is aligned and not NULL.
 inline int check_view(const char* op, const char* name, const void* data, int ndim, const int64_t* sizes,
                       const int64_t* strides, int min_nd, int bytes, int64_t* numel, Extent* ext) {
-    const std::string at = std::string(op) + ": " + name;
     if (ndim < min_nd || ndim > TLC_MAX_DIMS)
-        return set_error(TLC_ERR_INVALID_ARGUMENT,
-                         at + ": ndim must be " + std::to_string(min_nd) + ".." + std::to_string(TLC_MAX_DIMS));
+        return bad(op, name, (": ndim must be " + std::to_string(min_nd) + ".." + std::to_string(TLC_MAX_DIMS)).c_str());
     int64_t n = 1;
     bool empty = false;
     for (int i = 0; i < ndim; ++i) {
-        if (sizes[i] < 0) return set_error(TLC_ERR_INVALID_ARGUMENT, at + ": negative size");
-        if (strides[i] < 0) return set_error(TLC_ERR_INVALID_ARGUMENT, at + ": negative stride");
+        if (sizes[i] < 0) return bad(op, name, ": negative size");
+        if (strides[i] < 0) return bad(op, name, ": negative stride");
         empty = empty || sizes[i] == 0;
     }
     int64_t last = 0;
@@ -101,12 +104,12 @@ inline int check_view(const char* op, const char* name, const void* data, int nd
         int64_t step;
         if (__builtin_mul_overflow(n, sizes[i], &n) || __builtin_mul_overflow(sizes[i] - 1, strides[i], &step) ||
             __builtin_add_overflow(last, step, &last) || n > INT64_MAX / 16 || last > INT64_MAX / 16)
-            return set_error(TLC_ERR_INVALID_ARGUMENT, at + ": too large");
+            return bad(op, name, ": too large");
     }
     *numel = empty ? 0 : n;
     if (!empty) {
-        if (!data) return set_error(TLC_ERR_INVALID_ARGUMENT, at + ": NULL data");
-        if (!aligned_to(data, (size_t)bytes)) return set_error(TLC_ERR_INVALID_ARGUMENT, at + ": misaligned data");
+        if (!data) return bad(op, name, ": NULL data");
+        if (!aligned_to(data, (size_t)bytes)) return bad(op, name, ": misaligned data");
     }
     ext->lo = reinterpret_cast<uintptr_t>(data);
     ext->hi = empty ? ext->lo : ext->lo + (uintptr_t)(last + 1) * (uintptr_t)bytes;
@@ -133,7 +136,7 @@ struct RowView {
 };
 
 inline int row_view(const tlc_tensor* t, const char* op, const char* name, RowView& v) {
-    if (!t) return set_error(TLC_ERR_INVALID_ARGUMENT, std::string(op) + ": " + name + " is NULL");
+    if (!t) return bad(op, name, " is NULL");
     TLC_TRY(check_view(op, name, t->data, t->ndim, t->sizes, t->strides, 1, 4, &v.numel, &v.ext));
     v.data = t->data;
     v.cols = t->sizes[t->ndim - 1];
@@ -143,7 +146,7 @@ inline int row_view(const tlc_tensor* t, const char* op, const char* name, RowVi
         v.rows = 1;
         for (int i = 0; i + 1 < t->ndim; ++i)
             if (__builtin_mul_overflow(v.rows, t->sizes[i], &v.rows))
-                return set_error(TLC_ERR_INVALID_ARGUMENT, std::string(op) + ": " + name + ": too large");
+                return bad(op, name, ": too large");
     }
     v.map = merge_rows(t->ndim - 1, t->sizes, t->strides);
     return TLC_OK;
@@ -168,22 +171,20 @@ inline int unit_rows(const tlc_tensor* t, RowView& v, RowScratch& sc) {
 // A float input or output of exactly this shape; `contiguous` for outputs.
 inline int shaped(const tlc_tensor* t, const char* op, const char* name, int nd, const int64_t* sizes,
                   bool contiguous, Extent* ext) {
-    const std::string at = std::string(op) + ": " + name;
-    if (!t) return set_error(TLC_ERR_INVALID_ARGUMENT, at + " is NULL");
+    if (!t) return bad(op, name, " is NULL");
     bool same = t->ndim == nd;
     for (int i = 0; same && i < nd; ++i) same = t->sizes[i] == sizes[i];
-    if (!same) return set_error(TLC_ERR_INVALID_ARGUMENT, at + ": wrong shape");
+    if (!same) return bad(op, name, ": wrong shape");
     int64_t n;
     TLC_TRY(check_view(op, name, t->data, t->ndim, t->sizes, t->strides, 0, 4, &n, ext));
     if (contiguous && !dense_strides(nd, t->sizes, t->strides))
-        return set_error(TLC_ERR_INVALID_ARGUMENT, at + " must be contiguous");
+        return bad(op, name, " must be contiguous");
     return TLC_OK;
 }
 
 inline int index_view(const tlc_index* t, const char* op, const char* name, TokenRef& r, int64_t* numel, Extent* ext) {
-    const std::string at = std::string(op) + ": " + name;
-    if (!t) return set_error(TLC_ERR_INVALID_ARGUMENT, at + " is NULL");
-    if (t->bits != 32 && t->bits != 64) return set_error(TLC_ERR_INVALID_ARGUMENT, at + ": bits must be 32 or 64");
+    if (!t) return bad(op, name, " is NULL");
+    if (t->bits != 32 && t->bits != 64) return bad(op, name, ": bits must be 32 or 64");
     TLC_TRY(check_view(op, name, t->data, t->ndim, t->sizes, t->strides, 0, t->bits / 8, numel, ext));
     r.data = t->data;
     r.wide = t->bits == 64;

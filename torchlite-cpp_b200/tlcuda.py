@@ -12,7 +12,9 @@ binding works but every call raises: there is no fallback path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
+import struct
 
 import numpy as np
 
@@ -59,7 +61,7 @@ class Index(ctypes.Structure):
 # Every symbol include/tlc.h declares, with its ctypes signature.
 _P = ctypes.POINTER
 _T = _P(Tensor)
-_I = _P(Index)
+_B = ctypes.c_void_p  # a tlc_tensor or tlc_index given as the bytes of the struct
 _v, _i, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 SIGNATURES = {
     "tlc_version": ([], _i),
@@ -103,12 +105,12 @@ SIGNATURES = {
     "tlc_flash_attention": ([_T, _T, _T, ctypes.c_float, _T, _T, _i, _v], _i),
     "tlc_flash_attention_backward": ([_T, _T, _T, _T, _T, _T, ctypes.c_float, _T, _T, _T, _i, _v],
                                      _i),
-    "tlc_layer_norm": ([_T, _T, _T, ctypes.c_float, _T, _T, _v], _i),
-    "tlc_layer_norm_backward": ([_T, _T, _T, _T, _T, _T, _T, _i, _v], _i),
-    "tlc_embedding": ([_T, _I, ctypes.c_float, _T, _v], _i),
-    "tlc_embedding_backward": ([_T, _I, ctypes.c_float, _T, _i, _v], _i),
-    "tlc_token_logprobs": ([_T, _I, ctypes.c_float, _T, _T, _T, _i, _T, _I, _v], _i),
-    "tlc_token_logprobs_backward": ([_T, _I, _T, _T, _T, _T, ctypes.c_float, _T, _v], _i),
+    "tlc_layer_norm": ([_B, _B, _B, ctypes.c_float, _B, _B, _v], _i),
+    "tlc_layer_norm_backward": ([_B, _B, _B, _B, _B, _B, _B, _i, _v], _i),
+    "tlc_embedding": ([_B, _B, ctypes.c_float, _B, _v], _i),
+    "tlc_embedding_backward": ([_B, _B, ctypes.c_float, _B, _i, _v], _i),
+    "tlc_token_logprobs": ([_B, _B, ctypes.c_float, _B, _B, _B, _i, _B, _B, _v], _i),
+    "tlc_token_logprobs_backward": ([_B, _B, _B, _B, _B, _B, ctypes.c_float, _B, _v], _i),
     "tlc_load_tlmd": ([ctypes.c_char_p, ctypes.c_int32, _T, _v], _i),
     "tlc_save_tlmd": ([ctypes.c_char_p, ctypes.c_int32, _T, _v], _i),
     "tlc_shard_range": ([_i64, _i, _i, _P(_i64), _P(_i64)], _i),
@@ -435,100 +437,138 @@ def flash_attention_backward(grad, q, k, v, out, lse, sm_scale, mode="exact", dq
 
 
 # ---- token models: layer norm, embedding, token log-probabilities ------------------------
-# These check what the C ABI cannot see (types, and that every tensor is on the
-# current device) and raise ValueError; shapes and strides are checked there.
+# Small calls of these are bound by what Python does for them, so a view is packed into the
+# bytes of its struct in one step, and the device is looked up once a call.  They check what the
+# C ABI cannot see (types, and that every tensor is on the current device) and raise ValueError;
+# shapes and strides are checked there.  Each takes stream= (a torch stream; None: the current one).
 
-_SHAPE = ctypes.c_int64 * MAX_DIMS
-
-
-def _dev_view(t, name):
-    """tlc_tensor of a float32 CUDA tensor on the current device (None stays None)."""
-    import torch
-    if t is None:
-        return None
-    if t.dtype != torch.float32:
-        raise ValueError(f"{name}: libtl_cuda computes in float32, not {t.dtype}")
-    _on_current(t, name)
-    return Tensor(t.data_ptr(), t.dim(), _SHAPE(*t.shape), _SHAPE(*t.stride()))
+# tlc_tensor and tlc_index by rank: data, ndim (for an index with the bits in its upper half),
+# sizes and strides, padded to MAX_DIMS.
+_PACK = [struct.Struct(f"=QQ{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}x").pack
+         for n in range(MAX_DIMS + 1)]
 
 
-def _index_view(t, name):
-    """tlc_index of an int32 or int64 CUDA tensor on the current device."""
-    import torch
-    if t is None:
-        return None
-    if t.dtype is not torch.int64 and t.dtype is not torch.int32:
-        raise ValueError(f"{name}: int32 or int64, not {t.dtype}")
-    _on_current(t, name)
-    return Index(t.data_ptr(), t.dim(), 64 if t.dtype is torch.int64 else 32, _SHAPE(*t.shape),
-                 _SHAPE(*t.stride()))
-
-
-def _on_current(t, name):
-    import torch
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+def _refuse(t, dev, name, kinds):
+    if t.dtype not in kinds:
+        raise ValueError(f"{name}: {' or '.join(str(k)[6:] for k in kinds)}, not {t.dtype}")
     if t.dim() > MAX_DIMS:
         raise ValueError(f"{name}: at most {MAX_DIMS} dims")
+    raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
 
 
-def _new(like, shape, dtype=None):
-    import torch
-    return torch.empty(shape, dtype=dtype or torch.float32, device=like.device)
+def _fview(t, dev, name):
+    """The tlc_tensor of a float32 CUDA tensor on device `dev` as bytes (None stays None)."""
+    if t is None:
+        return None
+    n = t.dim()
+    if t.dtype is not _torch.float32 or not t.is_cuda or t.get_device() != dev or n > MAX_DIMS:
+        _refuse(t, dev, name, (_torch.float32,))
+    return _PACK[n](t.data_ptr(), n, *t.shape, *t.stride())
 
 
-def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None, stats=None, need_stats=True,
-               stream=None):
+def _iview(t, dev, name):
+    """The tlc_index of an int32 or int64 CUDA tensor on device `dev` as bytes."""
+    if t is None:
+        return None
+    n = t.dim()
+    bits = 64 if t.dtype is _torch.int64 else 32
+    if (bits == 32 and t.dtype is not _torch.int32) or not t.is_cuda or t.get_device() != dev or n > MAX_DIMS:
+        _refuse(t, dev, name, (_torch.int32, _torch.int64))
+    return _PACK[n](t.data_ptr(), n | bits << 32, *t.shape, *t.stride())
+
+
+_torch = None
+
+
+def _device(x):
+    """The current CUDA device (-1, which no tensor is on, where `x` is on none)."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch.cuda.current_device() if x.is_cuda else -1
+
+
+def _on_stream(f):
+    """Gives `f` the argument `stream`: f runs with it as the current stream, so what f
+    allocates belongs to the stream that writes it."""
+    @functools.wraps(f)
+    def call(*args, stream=None, **kw):
+        if stream is None:
+            return f(*args, **kw)
+        import torch
+        with torch.cuda.stream(stream):
+            return f(*args, **kw)
+    return call
+
+
+def _current(dev):
+    return _torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _like(x):
+    """An uninitialised contiguous tensor of x's shape, type and device."""
+    return _torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
+@_on_stream
+def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None, stats=None, need_stats=True):
     """Layer norm over the last dim: returns (out, stats), stats [..., 2] = (mean, rstd) of
     each row, what the backward needs (None with need_stats=False)."""
+    dev = _device(x)
     if x.dim() == 0:
         raise ValueError("layer_norm: x must be at least 1-D")
+    vx = _fview(x, dev, "x")
     if out is None:
-        out = _new(x, x.shape)
+        out = _like(x)
     if stats is None and need_stats:
-        stats = _new(x, (*x.shape[:-1], 2))
-    _check(lib().tlc_layer_norm(_dev_view(x, "x"), _dev_view(weight, "weight"),
-                                _dev_view(bias, "bias"), eps, _dev_view(out, "out"),
-                                _dev_view(stats, "stats"), _stream_ptr(stream)))
+        stats = x.new_empty((*x.shape[:-1], 2))
+    _check(lib().tlc_layer_norm(vx, _fview(weight, dev, "weight"), _fview(bias, dev, "bias"), eps,
+                                _fview(out, dev, "out"), _fview(stats, dev, "stats"),
+                                _current(dev)))
     return out, stats
 
 
+@_on_stream
 def layer_norm_backward(grad, x, stats, weight=None, need=(True, True, True), dx=None,
-                        dweight=None, dbias=None, accumulate=False, stream=None):
+                        dweight=None, dbias=None, accumulate=False):
     """Gradients of layer_norm: (dx, dweight, dbias), None where not requested.  With
     accumulate, given outputs receive their old values plus the gradient."""
+    dev = _device(x)
     if x.dim() == 0:
         raise ValueError("layer_norm_backward: x must be at least 1-D")
-    outs = []
-    for want, t, shape in zip(need, (dx, dweight, dbias), (x.shape, x.shape[-1:], x.shape[-1:])):
-        if want and t is None:
-            if accumulate:
-                raise ValueError("layer_norm_backward: accumulate needs the outputs it adds to")
-            t = _new(x, shape)
-        outs.append(t if want else None)
+    if accumulate and any(w and t is None for w, t in zip(need, (dx, dweight, dbias))):
+        raise ValueError("layer_norm_backward: accumulate needs the outputs it adds to")
+    vx = _fview(x, dev, "x")
+    dx = (_like(x) if dx is None else dx) if need[0] else None
+    dweight = (x.new_empty(x.shape[-1]) if dweight is None else dweight) if need[1] else None
+    dbias = (x.new_empty(x.shape[-1]) if dbias is None else dbias) if need[2] else None
     _check(lib().tlc_layer_norm_backward(
-        _dev_view(grad, "grad"), _dev_view(x, "x"), _dev_view(stats, "stats"),
-        _dev_view(weight, "weight"), _dev_view(outs[0], "dx"), _dev_view(outs[1], "dweight"),
-        _dev_view(outs[2], "dbias"), int(accumulate), _stream_ptr(stream)))
-    return tuple(outs)
+        _fview(grad, dev, "grad"), vx, _fview(stats, dev, "stats"), _fview(weight, dev, "weight"),
+        _fview(dx, dev, "dx"), _fview(dweight, dev, "dweight"), _fview(dbias, dev, "dbias"),
+        int(accumulate), _current(dev)))
+    return dx, dweight, dbias
 
 
-def embedding(weight, tokens, scale=1.0, out=None, stream=None):
+@_on_stream
+def embedding(weight, tokens, scale=1.0, out=None):
     """out[i] = scale * weight[tokens[i]]; token -1 (padding) gives zeros, any other token
     outside the table a row of NaN."""
+    dev = _device(weight)
     if weight.dim() != 2:
         raise ValueError("embedding: weight must be 2-D")
+    vt, vw = _iview(tokens, dev, "tokens"), _fview(weight, dev, "weight")
     if out is None:
-        out = _new(weight, (*tokens.shape, weight.shape[1]))
-    _check(lib().tlc_embedding(_dev_view(weight, "weight"), _index_view(tokens, "tokens"), scale,
-                               _dev_view(out, "out"), _stream_ptr(stream)))
+        out = weight.new_empty((*tokens.shape, weight.shape[1]))
+    _check(lib().tlc_embedding(vw, vt, scale, _fview(out, dev, "out"), _current(dev)))
     return out
 
 
-def embedding_backward(grad, tokens, rows=None, scale=1.0, dweight=None, accumulate=False,
-                       stream=None):
+@_on_stream
+def embedding_backward(grad, tokens, rows=None, scale=1.0, dweight=None, accumulate=False):
     """The table's gradient [rows, D]: sums of grad over the positions of each token, times
     scale.  With accumulate they are added to `dweight`."""
+    dev = _device(grad)
     if grad.dim() == 0:
         raise ValueError("embedding_backward: grad must be at least 1-D")
     if dweight is None:
@@ -536,55 +576,59 @@ def embedding_backward(grad, tokens, rows=None, scale=1.0, dweight=None, accumul
             raise ValueError("embedding_backward: accumulate needs the dweight it adds to")
         if rows is None:
             raise ValueError("embedding_backward: rows (the table's length) or dweight is needed")
-        dweight = _new(grad, (rows, grad.shape[-1]))
-    elif rows is not None and rows != dweight.shape[0]:
+        dweight = grad.new_empty((rows, grad.shape[-1]))
+    elif rows is not None and (dweight.dim() != 2 or rows != dweight.shape[0]):
         raise ValueError("embedding_backward: dweight has another number of rows")
-    _check(lib().tlc_embedding_backward(_dev_view(grad, "grad"), _index_view(tokens, "tokens"),
-                                        scale, _dev_view(dweight, "dweight"), int(accumulate),
-                                        _stream_ptr(stream)))
+    vg, vt = _fview(grad, dev, "grad"), _iview(tokens, dev, "tokens")
+    _check(lib().tlc_embedding_backward(vg, vt, scale, _fview(dweight, dev, "dweight"),
+                                        int(accumulate), _current(dev)))
     return dweight
 
 
-def token_logprobs(logits, tokens=None, scale=1.0, top=0, need_entropy=True, need_stats=True,
-                   stream=None):
+@_on_stream
+def token_logprobs(logits, tokens=None, scale=1.0, top=0, need_entropy=True, need_stats=True):
     """Of p = softmax(scale * logits) over the last dim: (logprobs, entropy, stats,
     top_logprobs, top_tokens), None where not requested.  logprobs: log p of the given tokens
     (0 for token -1); stats: what token_logprobs_backward needs; top_*: the `top` (at most 32)
     most likely tokens in order, of the type of `tokens` (int64 without tokens)."""
-    import torch
+    dev = _device(logits)
     if logits.dim() == 0:
         raise ValueError("token_logprobs: logits must be at least 1-D")
+    vx, vt = _fview(logits, dev, "logits"), _iview(tokens, dev, "tokens")
     lead = logits.shape[:-1]
-    logp = _new(logits, lead) if tokens is not None else None
-    entropy = _new(logits, lead) if need_entropy else None
-    stats = _new(logits, (*lead, 2)) if need_stats else None
+    logp = logits.new_empty(lead) if tokens is not None else None
+    entropy = logits.new_empty(lead) if need_entropy else None
+    stats = logits.new_empty((*lead, 2)) if need_stats else None
     top_logp = top_tokens = None
     if top:
-        top_logp = _new(logits, (*lead, top))
-        top_tokens = _new(logits, (*lead, top), tokens.dtype if tokens is not None else torch.int64)
+        lead = (*lead, top)
+        top_logp = logits.new_empty(lead)
+        top_tokens = (logits.new_empty(lead, dtype=_torch.int64) if tokens is None else
+                      tokens.new_empty(lead))
     _check(lib().tlc_token_logprobs(
-        _dev_view(logits, "logits"), _index_view(tokens, "tokens"), scale,
-        _dev_view(logp, "logprobs"), _dev_view(entropy, "entropy"), _dev_view(stats, "stats"), top,
-        _dev_view(top_logp, "top_logprobs"), _index_view(top_tokens, "top_tokens"),
-        _stream_ptr(stream)))
+        vx, vt, scale, _fview(logp, dev, "logprobs"), _fview(entropy, dev, "entropy"),
+        _fview(stats, dev, "stats"), top, _fview(top_logp, dev, "top_logprobs"),
+        _iview(top_tokens, dev, "top_tokens"), _current(dev)))
     return logp, entropy, stats, top_logp, top_tokens
 
 
+@_on_stream
 def token_logprobs_backward(logits, tokens, stats, grad_logprobs=None, grad_entropy=None,
-                            entropy=None, scale=1.0, out=None, stream=None):
+                            entropy=None, scale=1.0, out=None):
     """The gradient to the logits from those of logprobs and entropy (with grad_entropy the
     forward's entropy is needed).  `out` may be the (contiguous) logits themselves."""
+    dev = _device(logits)
     if logits.dim() == 0:
         raise ValueError("token_logprobs_backward: logits must be at least 1-D")
     if grad_entropy is not None and entropy is None:
         raise ValueError("token_logprobs_backward: grad_entropy needs the forward's entropy")
+    vx, vt = _fview(logits, dev, "logits"), _iview(tokens, dev, "tokens")
     if out is None:
-        out = _new(logits, logits.shape)
+        out = _like(logits)
     _check(lib().tlc_token_logprobs_backward(
-        _dev_view(logits, "logits"), _index_view(tokens, "tokens"), _dev_view(stats, "stats"),
-        _dev_view(entropy, "entropy"), _dev_view(grad_logprobs, "grad_logprobs"),
-        _dev_view(grad_entropy, "grad_entropy"), scale, _dev_view(out, "out"),
-        _stream_ptr(stream)))
+        vx, vt, _fview(stats, dev, "stats"), _fview(entropy, dev, "entropy"),
+        _fview(grad_logprobs, dev, "grad_logprobs"), _fview(grad_entropy, dev, "grad_entropy"),
+        scale, _fview(out, dev, "out"), _current(dev)))
     return out
 
 
