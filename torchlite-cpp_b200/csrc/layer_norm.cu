@@ -130,34 +130,95 @@ struct LnBwd {
     int accumulate;
 };
 
-// As the forward; each thread keeps the same columns for every row of its
-// block, so the sums for dw and db stay in its registers until the end.
-template <int VEC, int VPT, int THREADS>
-__global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) ln_bwd_kernel(LnBwd p) {
-    constexpr int RPB = THREADS == 32 ? 8 : 1;
-    extern __shared__ float sums[];  // THREADS == 32: [8][2][D]
-    __shared__ float red[2][64];
-    const int t = THREADS == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const int sub = THREADS == 32 ? (threadIdx.x >> 5) : 0;
+// One block an SM, 8 warps; W warps a row, 8 / W rows at a time.  Each lane
+// keeps the same columns for every row, so the sums for dw and db stay in its
+// registers until the end.  The rows come through a ring of STAGES rows of x
+// and g in shared memory, filled by asynchronous copies: a thread copies just
+// what it reads itself, so the ring needs no barrier, and rows far enough
+// ahead are always in flight although the registers allow only 8 warps.
+constexpr int BT = 256;
+
+template <int VEC>
+__device__ __forceinline__ void copy_async(float* dst, const float* src) {
+    const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+    if constexpr (VEC == 4)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Rows of x and g kept in shared memory: what 192 KB hold, at most 8.
+template <int VEC, int VPT>
+constexpr int ring_stages() {
+    const int n = 192 * 1024 / (BT * VPT * VEC * 4 * 2);
+    return n < 8 ? n : 8;
+}
+
+template <int VEC, int VPT, int W>
+__global__ void __launch_bounds__(BT, 1) ln_bwd_kernel(LnBwd p) {
+    constexpr int S = ring_stages<VEC, VPT>();
+    constexpr int GROUPS = BT / 32 / W, THREADS = 32 * W;
+    extern __shared__ __align__(16) float ring[];  // [S][2][VPT][BT][VEC], then [GROUPS][2][D]
+    __shared__ float red[2][GROUPS][2 * W];
+    const int group = threadIdx.x / THREADS, t = threadIdx.x % THREADS, lane = threadIdx.x & 31;
     const float inv = 1.0f / (float)p.D;
-    float aw[VPT][VEC], ab[VPT][VEC];
+    float aw[VPT][VEC], ab[VPT][VEC], w[VPT][VEC];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+    for (int i = 0; i < VPT; ++i) {
+        const int j = (t + i * THREADS) * VEC;
+        if (p.w && j < p.D) load_vec<VEC>(p.w + j, w[i]);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) aw[i][k] = ab[i][k] = 0.0f;
-    int turn = 0;
-    for (int64_t r = (int64_t)blockIdx.x * RPB + sub; r < p.rows; r += (int64_t)gridDim.x * RPB) {
-        const float* xr = p.x + p.xm.offset(r);
-        const float* gr = p.g + p.gm.offset(r);
-        const float* st = p.stats + p.sm.offset(r);
-        const float mean = st[0], rstd = st[1];
+        for (int k = 0; k < VEC; ++k) {
+            aw[i][k] = ab[i][k] = 0.0f;
+            if (!p.w || j >= p.D) w[i][k] = 1.0f;
+        }
+    }
+    const int64_t step = (int64_t)gridDim.x * GROUPS;
+    const int64_t r0 = blockIdx.x + (int64_t)gridDim.x * group;
+    auto slot = [&](int stage, int which, int i) {
+        return ring + ((((stage * 2 + which) * VPT + i) * BT) + threadIdx.x) * VEC;
+    };
+    auto fetch = [&](int64_t r, int stage) {
+        if (r < p.rows) {
+            const float* xr = p.x + p.xm.offset(r);
+            const float* gr = p.g + p.gm.offset(r);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int j = (t + i * THREADS) * VEC;
+                if (j < p.D) {
+                    copy_async<VEC>(slot(stage, 0, i), xr + j);
+                    copy_async<VEC>(slot(stage, 1, i), gr + j);
+                }
+            }
+        }
+        copies_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < S; ++s) fetch(r0 + s * step, s);
+    int stage = 0, turn = 0;
+    float next[2] = {0.0f, 0.0f};
+    auto fetch_stats = [&](int64_t r) {
+        if (r < p.rows) {
+            const float* st = p.stats + p.sm.offset(r);
+            next[0] = st[0], next[1] = st[1];
+        }
+    };
+    fetch_stats(r0);
+    for (int64_t r = r0; r < p.rows; r += step) {
+        const float mean = next[0], rstd = next[1];
+        fetch_stats(r + step);
+        copies_wait<S - 1>();
         float x[VPT][VEC], g[VPT][VEC];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int j = (t + i * THREADS) * VEC;
-            if (j < p.D) {
-                load_once<VEC>(xr + j, x[i]);
-                load_once<VEC>(gr + j, g[i]);
+            if ((t + i * THREADS) * VEC < p.D) {
+                load_vec<VEC>(slot(stage, 0, i), x[i]);
+                load_vec<VEC>(slot(stage, 1, i), g[i]);
             } else {
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) x[i][k] = mean, g[i][k] = 0.0f;
@@ -165,73 +226,66 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) ln_bwd_kernel(L
         }
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int j = (t + i * THREADS) * VEC;
-            float wv[VEC];
-            if (p.w && j < p.D) load_vec<VEC>(p.w + j, wv);
+        for (int i = 0; i < VPT; ++i)
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
                 x[i][k] = (x[i][k] - mean) * rstd;
                 aw[i][k] = fmaf(g[i][k], x[i][k], aw[i][k]);
                 ab[i][k] += g[i][k];
-                if (p.w && j < p.D) g[i][k] *= wv[k];
+                g[i][k] *= w[i][k];
                 s[0] += g[i][k];
                 s[1] = fmaf(g[i][k], x[i][k], s[1]);
             }
-        }
-        if (p.dx) {
-            group_sum<THREADS>(s, red[turn]);
+        fetch(r + S * step, stage);  // into the row just read
+        stage = stage + 1 == S ? 0 : stage + 1;
+        if (!p.dx) continue;
+        warp_sum(s);
+        if constexpr (W > 1) {
+            float* mine = red[turn][group];
+            if (lane == 0) mine[2 * (t >> 5)] = s[0], mine[2 * (t >> 5) + 1] = s[1];
+            asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(THREADS) : "memory");
+            s[0] = s[1] = 0.0f;
+#pragma unroll
+            for (int q = 0; q < W; ++q) s[0] += mine[2 * q], s[1] += mine[2 * q + 1];
             turn ^= 1;
-            const float c0 = s[0] * inv, c1 = s[1] * inv;
-            float* dr = p.dx + r * p.D;
+        }
+        const float c0 = s[0] * inv, c1 = s[1] * inv;
+        float* dr = p.dx + r * p.D;
 #pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                const int j = (t + i * THREADS) * VEC;
-                if (j < p.D) {
-                    float y[VEC], old[VEC];
-                    if (p.accumulate) load_vec<VEC>(dr + j, old);
+        for (int i = 0; i < VPT; ++i) {
+            const int j = (t + i * THREADS) * VEC;
+            if (j < p.D) {
+                float y[VEC], old[VEC];
+                if (p.accumulate) load_vec<VEC>(dr + j, old);
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) {
-                        y[k] = __fmul_rn(rstd, g[i][k] - fmaf(x[i][k], c1, c0));
-                        if (p.accumulate) y[k] = __fadd_rn(y[k], old[k]);  // the gradient rounded, then added
-                    }
-                    store_vec<VEC>(dr + j, y);
+                for (int k = 0; k < VEC; ++k) {
+                    y[k] = __fmul_rn(rstd, g[i][k] - fmaf(x[i][k], c1, c0));
+                    if (p.accumulate) y[k] = __fadd_rn(y[k], old[k]);  // the gradient rounded, then added
                 }
+                store_vec<VEC>(dr + j, y);
             }
         }
     }
+    copies_wait<0>();
     if (!p.part) return;
     float* part = p.part + (int64_t)blockIdx.x * 2 * p.D;
-    if constexpr (THREADS == 32) {
+    float* sums = GROUPS > 1 ? ring + (int64_t)group * 2 * p.D : part;
+    __syncthreads();  // nobody reads the ring any more
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int j = (t + i * THREADS) * VEC;
-            if (j < p.D) {
+    for (int i = 0; i < VPT; ++i) {
+        const int j = (t + i * THREADS) * VEC;
+        if (j < p.D) {
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    sums[(2 * sub) * p.D + j + k] = aw[i][k];
-                    sums[(2 * sub + 1) * p.D + j + k] = ab[i][k];
-                }
-            }
+            for (int k = 0; k < VEC; ++k) sums[j + k] = aw[i][k], sums[p.D + j + k] = ab[i][k];
         }
+    }
+    if constexpr (GROUPS > 1) {
         __syncthreads();
-        for (int j = threadIdx.x; j < 2 * p.D; j += blockDim.x) {
+        for (int j = threadIdx.x; j < 2 * p.D; j += BT) {
             float a = 0.0f;
 #pragma unroll
-            for (int q = 0; q < RPB; ++q) a += sums[q * 2 * p.D + j];
+            for (int q = 0; q < GROUPS; ++q) a += ring[q * 2 * p.D + j];
             part[j] = a;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int j = (t + i * THREADS) * VEC;
-            if (j < p.D) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    part[j + k] = aw[i][k];
-                    part[p.D + j + k] = ab[i][k];
-                }
-            }
         }
     }
 }
@@ -282,22 +336,23 @@ __global__ void __launch_bounds__(256) ln_bwd_cols_kernel(LnBwd p, int64_t rows_
     part[p.D + j] = b;
 }
 
-// dw = sum of the blocks' sums in their order: 32 columns a block, 8 warps
+// dw = sum of the blocks' sums in their order: 32 columns a block, 16 warps
 // over the parts.  Columns [0, D) are dw's, [D, 2D) db's.
-__global__ void __launch_bounds__(256) ln_bwd_finish_kernel(const float* __restrict__ part, int parts, int D,
+__global__ void __launch_bounds__(512) ln_bwd_finish_kernel(const float* __restrict__ part, int parts, int D,
                                                             float* dw, float* db, int accumulate) {
-    __shared__ float red[8][33];
+    __shared__ float red[16][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t j = (int64_t)blockIdx.x * 32 + lane;
     float a = 0.0f;
     if (j < 2 * (int64_t)D)
-        for (int q = warp; q < parts; q += 8) a += part[(int64_t)q * 2 * D + j];
+#pragma unroll 5
+        for (int q = warp; q < parts; q += 16) a += part[(int64_t)q * 2 * D + j];
     red[warp][lane] = a;
     __syncthreads();
     if (warp == 0 && j < 2 * (int64_t)D) {
         a = 0.0f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) a += red[q][lane];
+        for (int q = 0; q < 16; ++q) a += red[q][lane];
         float* out = j < D ? (dw ? dw + j : nullptr) : (db ? db + (j - D) : nullptr);
         if (out) *out = accumulate ? *out + a : a;
     }
@@ -338,60 +393,51 @@ int pick_fwd(const LnFwd& p, cudaStream_t s) {
             return launch_fwd<VEC, 32, 32>(p, s);
         }
     }
-    if (n <= 256 * 2) return launch_fwd<VEC, 2, 256>(p, s);
-    if (n <= 256 * 4) return launch_fwd<VEC, 4, 256>(p, s);
-    if (n <= 512 * 4) return launch_fwd<VEC, 4, 512>(p, s);
-    if (n <= 1024 * 4) return launch_fwd<VEC, 4, 1024>(p, s);
-    if constexpr (VEC == 1) {
-        if (n <= 1024 * 8) return launch_fwd<VEC, 8, 1024>(p, s);
-        if (n <= 1024 * 16) return launch_fwd<VEC, 16, 1024>(p, s);
+    // 16 to 32 values a thread: many small blocks keep more rows in flight than few large ones
+    if constexpr (VEC == 4) {
+        if (n <= 128 * 4) return launch_fwd<4, 4, 128>(p, s);
+        if (n <= 256 * 4) return launch_fwd<4, 4, 256>(p, s);
+        if (n <= 256 * 8) return launch_fwd<4, 8, 256>(p, s);
+        if (n <= 512 * 8) return launch_fwd<4, 8, 512>(p, s);
+        if (n <= 1024 * 8) return launch_fwd<4, 8, 1024>(p, s);
+    } else {
+        if (n <= 128 * 16) return launch_fwd<1, 16, 128>(p, s);
+        if (n <= 256 * 16) return launch_fwd<1, 16, 256>(p, s);
+        if (n <= 256 * 24) return launch_fwd<1, 24, 256>(p, s);
+        if (n <= 512 * 16) return launch_fwd<1, 16, 512>(p, s);
+        if (n <= 512 * 24) return launch_fwd<1, 24, 512>(p, s);
+        if (n <= 1024 * 16) return launch_fwd<1, 16, 1024>(p, s);
     }
     ln_fwd_long_kernel<<<(unsigned)std::min<int64_t>(p.rows, INT32_MAX), 1024, 0, s>>>(p);
     count_launch();
     return check_launch(kFwd);
 }
 
-template <int VEC, int VPT, int THREADS>
+constexpr int kRingMax = 8192;  // 32 columns a lane of 8 warps
+
+template <int VEC, int VPT, int W>
 int launch_bwd(const LnBwd& p, int grid, cudaStream_t s) {
-    const size_t smem = THREADS == 32 && p.part ? sizeof(float) * 16 * (size_t)p.D : 0;
+    const size_t ring = sizeof(float) * 2 * BT * VPT * VEC * ring_stages<VEC, VPT>();
     static DeviceOnce once;
-    if (smem)
-        TLC_TRY(smem_limit_once(once, ln_bwd_kernel<VEC, VPT, THREADS>, (int)(sizeof(float) * 16 * 1024)));
-    ln_bwd_kernel<VEC, VPT, THREADS><<<grid, THREADS == 32 ? 256 : THREADS, smem, s>>>(p);
+    TLC_TRY(smem_limit_once(once, ln_bwd_kernel<VEC, VPT, W>, (int)ring));
+    ln_bwd_kernel<VEC, VPT, W><<<grid, BT, ring, s>>>(p);
     count_launch();
     return check_launch(kBwd);
 }
 
-// The rows a block of the register kernels takes at once (0: the row is too long).
-int bwd_threads(int D, int vec) {
-    const int n = (D + vec - 1) / vec;
-    if (n * vec <= (vec == 4 ? 1024 : 512)) return 32;
-    const int per = vec == 4 ? 4 : 16;
-    if (n <= 128 * per) return 128;
-    if (n <= 256 * per) return 256;
-    if (n <= 512 * per) return 512;
-    return 0;
-}
-
+// 4 to 32 columns a lane; a row for one warp up to 1024 columns, then for 2, 4, 8.
 template <int VEC>
-int pick_bwd(const LnBwd& p, int threads, int grid, cudaStream_t s) {
-    const int n = (p.D + VEC - 1) / VEC;
-    constexpr int PER = VEC == 4 ? 4 : 16;
-    if (threads == 32) {
-        if (n <= 32) return launch_bwd<VEC, 1, 32>(p, grid, s);
-        if (n <= 64) return launch_bwd<VEC, 2, 32>(p, grid, s);
-        if (n <= 128) return launch_bwd<VEC, 4, 32>(p, grid, s);
-        if constexpr (VEC == 4) {
-            if (n <= 192) return launch_bwd<VEC, 6, 32>(p, grid, s);
-            return launch_bwd<VEC, 8, 32>(p, grid, s);
-        } else {
-            if (n <= 256) return launch_bwd<VEC, 8, 32>(p, grid, s);
-            return launch_bwd<VEC, 16, 32>(p, grid, s);
-        }
-    }
-    if (threads == 128) return launch_bwd<VEC, PER, 128>(p, grid, s);
-    if (threads == 256) return launch_bwd<VEC, PER, 256>(p, grid, s);
-    return launch_bwd<VEC, PER, 512>(p, grid, s);
+int pick_bwd(const LnBwd& p, int grid, cudaStream_t s) {
+    if (p.D <= 128) return launch_bwd<VEC, 4 / VEC, 1>(p, grid, s);
+    if (p.D <= 256) return launch_bwd<VEC, 8 / VEC, 1>(p, grid, s);
+    if (p.D <= 512) return launch_bwd<VEC, 16 / VEC, 1>(p, grid, s);
+    if (p.D <= 768) return launch_bwd<VEC, 24 / VEC, 1>(p, grid, s);
+    if (p.D <= 1024) return launch_bwd<VEC, 32 / VEC, 1>(p, grid, s);
+    if (p.D <= 1536) return launch_bwd<VEC, 24 / VEC, 2>(p, grid, s);
+    if (p.D <= 2048) return launch_bwd<VEC, 32 / VEC, 2>(p, grid, s);
+    if (p.D <= 4096) return launch_bwd<VEC, 32 / VEC, 4>(p, grid, s);
+    if (p.D <= 6144) return launch_bwd<VEC, 24 / VEC, 8>(p, grid, s);
+    return launch_bwd<VEC, 32 / VEC, 8>(p, grid, s);
 }
 
 // A weight or bias: NULL, or a 1-D tensor of length D with stride 1 (a copy in `sc` otherwise).
@@ -519,18 +565,15 @@ extern "C" int tlc_layer_norm_backward(const tlc_tensor* grad, const tlc_tensor*
     const bool sums = dweight || dbias;
     const bool vec = p.D % 4 == 0 && vx.map.multiple_of(4) && vg.map.multiple_of(4) && aligned_to(p.x, 16) &&
                      aligned_to(p.g, 16) && aligned_to(p.dx, 16) && aligned_to(p.w, 16);
-    const int threads = bwd_threads(p.D, vec ? 4 : 1);
     const int sms = sm_count();
     int parts = 0;
-    if (threads) {
-        const int rpb = threads == 32 ? 8 : 1;
-        const int64_t per_sm = threads == 32 ? 2 : std::max(1, 512 / threads);
-        parts = (int)std::min<int64_t>((p.rows + rpb - 1) / rpb, (int64_t)sms * per_sm);
+    if (p.D <= kRingMax) {
+        parts = (int)std::min<int64_t>(p.rows, sms);
         if (sums) {
             TLC_TRY(scratch_alloc(&cp.p, sizeof(float) * 2 * (size_t)p.D * (size_t)parts, s));
             p.part = cp.f();
         }
-        TLC_TRY(vec ? pick_bwd<4>(p, threads, parts, s) : pick_bwd<1>(p, threads, parts, s));
+        TLC_TRY(vec ? pick_bwd<4>(p, parts, s) : pick_bwd<1>(p, parts, s));
     } else {
         if (dx) {
             ln_bwd_long_kernel<<<(unsigned)std::min<int64_t>(p.rows, INT32_MAX), 1024, 0, s>>>(p);
@@ -551,7 +594,7 @@ extern "C" int tlc_layer_norm_backward(const tlc_tensor* grad, const tlc_tensor*
     }
     if (sums) {
         const int64_t blocks = (2 * (int64_t)p.D + 31) / 32;
-        ln_bwd_finish_kernel<<<(unsigned)blocks, 256, 0, s>>>(p.part, parts, p.D, dweight ? dweight->data : nullptr,
+        ln_bwd_finish_kernel<<<(unsigned)blocks, 512, 0, s>>>(p.part, parts, p.D, dweight ? dweight->data : nullptr,
                                                              dbias ? dbias->data : nullptr, p.accumulate);
         count_launch();
         TLC_TRY(check_launch(kBwd));
