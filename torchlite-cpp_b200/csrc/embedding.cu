@@ -63,74 +63,159 @@ __global__ void __launch_bounds__(256) embed_kernel(EmbFwd p, int pieces) {
     }
 }
 
-// ---- the positions sorted by token ------------------------------------------------------
+// ---- the positions sorted by token, and the rows that stay zero ----------------------------
 //
-// A radix sort by one cluster of CL blocks, least digit first.  In each pass a
-// block counts the digits of its part of the list, the cluster exchanges the
-// counts through distributed shared memory, and the block scatters its part
-// tile by tile: a warp ranks its 32 * ITEMS consecutive keys by matching
-// digits across lanes, then the warps' counts are scanned digit by digit.
-// Stable at every level, and the result does not depend on timing.
+// One launch does both, so that the zeros of the table are written while eight
+// SMs sort.  Cluster 0 of CL blocks runs a radix sort, least digit first.  In
+// each pass a warp ranks its 32 * items consecutive keys by matching digits
+// across lanes, the warps' counts are scanned digit by digit, the cluster
+// exchanges the blocks' counts through distributed shared memory, and each key
+// goes to its place.  Stable at every level, and the result does not depend on
+// timing.  Up to CL * TILE positions the list stays in the blocks' shared
+// memory between passes; longer lists go through global memory tile by tile.
+// The other clusters share the rows: a cluster's blocks look through the
+// positions (each an eighth), mark its rows that occur in one another's shared
+// memory, and write zeros to the rest.
 
 constexpr int CL = 8;
 constexpr int SORT_T = 1024;
+constexpr int WARPS = SORT_T / 32;
 constexpr int ITEMS = 8;
 constexpr int MAX_BITS = 9;
 constexpr int BINS = 1 << MAX_BITS;
 constexpr int TILE = SORT_T * ITEMS;
+constexpr int ZROWS = 65536;  // rows whose marks a block holds at once
 
 struct SortArgs {
     TokenRef tok;
     int64_t rows;     // tokens outside [0, rows) get the key `rows`: behind all others
     int n;
     int bits, passes;  // digits of `bits` bits
-    uint2* a;          // [n] (key, position): even passes write here
-    uint2* b;          // [n]: odd passes
+    uint2* a;          // [n] (key, position), where even passes write
+    uint2* b;          // [n], odd passes
+    int* crossing;     // set to 0 here: the count of runs that cross chunks
+    float* dw;         // rows to fill with zeros (NULL: none)
+    int D, vec;        // vec: rows start on 16 bytes
+    int group_shift;   // rows are dealt to the blocks in groups of 2^group_shift, at least 2 KB each
 };
 
 struct SortSmem {
     uint32_t hist[BINS];           // this block's counts, read by the cluster
     uint32_t base[BINS];           // where this block's next key of a digit goes
-    uint32_t scan[BINS];
-    uint32_t warp[SORT_T / 32][BINS];
-    uint32_t wsum[32];
+    uint32_t warp[WARPS][BINS];    // a warp's counts, then where its keys go within the block's
+    uint32_t wsum[WARPS];
+    uint2 keys[TILE];              // the block's part of the list between passes
+};
+struct FillSmem {
+    uint32_t marks[ZROWS / 32];
 };
 
+__device__ __forceinline__ uint32_t cluster_addr(const void* local, uint32_t rank) {
+    return mapa(static_cast<uint32_t>(__cvta_generic_to_shared(local)), rank);
+}
 __device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* local, uint32_t rank) {
     uint32_t v;
-    const uint32_t addr = mapa(static_cast<uint32_t>(__cvta_generic_to_shared(local)), rank);
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(local, rank)) : "memory");
     return v;
 }
 
-__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(SORT_T) embed_sort_kernel(SortArgs p) {
-    extern __shared__ __align__(16) unsigned char raw[];
-    SortSmem& sm = *reinterpret_cast<SortSmem*>(raw);
+__device__ void sort_positions(const SortArgs& p, SortSmem& sm) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = (int)cluster_ctarank();
     const int per = (p.n + CL - 1) / CL;
     const int i0 = min(p.n, rank * per), i1 = min(p.n, i0 + per);
     const int bins = 1 << p.bits;
+    const bool one = per <= TILE;  // the block's part is one tile
+    const int items = min(ITEMS, (per + SORT_T - 1) / SORT_T);
+    if (rank == 0 && tid == 0) *p.crossing = 0;
+    uint2 kv[ITEMS];
+    uint32_t at[ITEMS];
     for (int pass = 0; pass < p.passes; ++pass) {
         const uint2* src = (pass & 1) ? p.a : p.b;  // pass 0 reads the tokens
         uint2* dst = (pass & 1) ? p.b : p.a;
+        const bool last = pass + 1 == p.passes;
         const int shift = pass * p.bits;
+        auto digit = [&](uint2 k) { return (k.x >> shift) & (uint32_t)(bins - 1); };
         auto load = [&](int i) -> uint2 {
-            if (pass > 0) return __ldcg(src + i);
-            const int64_t t = p.tok.get(i);
-            return make_uint2((uint32_t)(t >= 0 && t < p.rows ? t : p.rows), (uint32_t)i);
+            if (pass == 0) {
+                const int64_t t = p.tok.get(i);
+                return make_uint2((uint32_t)(t >= 0 && t < p.rows ? t : p.rows), (uint32_t)i);
+            }
+            return one ? sm.keys[i - i0] : __ldcg(src + i);
         };
-        for (int d = tid; d < BINS; d += SORT_T) sm.hist[d] = 0;
-        __syncthreads();
-        for (int i = i0 + tid; i < i1; i += SORT_T) atomicAdd(&sm.hist[(load(i).x >> shift) & (bins - 1)], 1u);
-        cluster_sync();
+        // a tile's keys, and each key's place among its warp's of the same digit
+        auto rank_tile = [&](int t0) {
+            for (int d = lane; d < bins; d += 32) sm.warp[warp][d] = 0;
+            const int w0 = t0 + warp * 32 * items + lane;
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k)
+                if (k < items && w0 + k * 32 < i1) kv[k] = load(w0 + k * 32);
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k) {
+                if (k >= items) break;
+                const bool in = w0 + k * 32 < i1;
+                // lanes past the end match nobody's digit
+                const uint32_t d = in ? digit(kv[k]) : (uint32_t)(BINS + lane);
+                const uint32_t peers = __match_any_sync(0xffffffffu, d);
+                const uint32_t old = in ? sm.warp[warp][d] : 0u;
+                __syncwarp();
+                if (in && lane == 31 - __clz(peers)) sm.warp[warp][d] = old + __popc(peers);
+                __syncwarp();
+                at[k] = old + __popc(peers & ((1u << lane) - 1u));
+            }
+            __syncthreads();
+        };
+        // the warps' counts of a digit -> the places of each warp's first; returns the block's count
+        auto scan_warps = [&](int d) -> uint32_t {
+            uint32_t c[WARPS], run = 0;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) c[w] = sm.warp[w][d];
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                sm.warp[w][d] = run;
+                run += c[w];
+            }
+            return run;
+        };
+        auto place_tile = [&](int t0) {
+            const int w0 = t0 + warp * 32 * items + lane;
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k) {
+                if (k < items && w0 + k * 32 < i1) {
+                    const uint32_t d = digit(kv[k]);
+                    const uint32_t to = sm.base[d] + sm.warp[warp][d] + at[k];
+                    if (one && !last) {
+                        const uint32_t owner = to / (uint32_t)per;
+                        asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(
+                                         cluster_addr(&sm.keys[to - owner * (uint32_t)per], owner)),
+                                     "r"(kv[k].x), "r"(kv[k].y)
+                                     : "memory");
+                    } else {
+                        dst[to] = kv[k];
+                    }
+                }
+            }
+        };
+        if (one) {
+            rank_tile(i0);
+            if (tid < bins) sm.hist[tid] = scan_warps(tid);
+        } else {
+            for (int d = tid; d < bins; d += SORT_T) sm.hist[d] = 0;
+            __syncthreads();
+            for (int i = i0 + tid; i < i1; i += SORT_T) atomicAdd(&sm.hist[digit(load(i))], 1u);
+        }
+        cluster_sync();  // counts in place; with one tile all keys are in registers as well
         // base[d] = keys of lower digits in the cluster + keys of d in lower blocks
         uint32_t total = 0, below = 0;
         if (tid < bins) {
-            for (int c = 0; c < CL; ++c) {
-                const uint32_t v = ld_cluster_u32(&sm.hist[tid], (uint32_t)c);
-                total += v;
-                if (c < rank) below += v;
+            uint32_t c[CL];
+#pragma unroll
+            for (int q = 0; q < CL; ++q) c[q] = ld_cluster_u32(&sm.hist[tid], (uint32_t)q);
+#pragma unroll
+            for (int q = 0; q < CL; ++q) {
+                total += c[q];
+                if (q < rank) below += c[q];
             }
         }
         uint32_t incl = total;
@@ -143,67 +228,104 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(SORT_T) embed_sort_
         __syncthreads();
         if (tid < bins) {
             uint32_t before = 0;
-            for (int w = 0; w < warp; ++w) before += sm.wsum[w];
+#pragma unroll
+            for (int w = 0; w < BINS / 32; ++w) before += w < warp ? sm.wsum[w] : 0u;
             sm.base[tid] = before + incl - total + below;
         }
         __syncthreads();
-        for (int t0 = i0; t0 < i1; t0 += TILE) {
-            for (int d = lane; d < bins; d += 32) sm.warp[warp][d] = 0;
-            __syncwarp();
-            uint2 kv[ITEMS];
-            uint32_t at[ITEMS];
-            const int w0 = t0 + warp * 32 * ITEMS;
-#pragma unroll
-            for (int k = 0; k < ITEMS; ++k) {
-                const int i = w0 + k * 32 + lane;
-                kv[k] = i < i1 ? load(i) : make_uint2(0u, 0u);
+        if (one) {
+            place_tile(i0);
+        } else {
+            for (int t0 = i0; t0 < i1; t0 += TILE) {
+                rank_tile(t0);
+                const uint32_t count = tid < bins ? scan_warps(tid) : 0u;
+                __syncthreads();
+                place_tile(t0);
+                __syncthreads();
+                if (tid < bins) sm.base[tid] += count;
             }
-#pragma unroll
-            for (int k = 0; k < ITEMS; ++k) {
-                const bool in = w0 + k * 32 + lane < i1;
-                // lanes past the end match nobody's digit
-                const uint32_t d = in ? (kv[k].x >> shift) & (uint32_t)(bins - 1) : (uint32_t)(BINS + lane);
-                const uint32_t peers = __match_any_sync(0xffffffffu, d);
-                const uint32_t old = in ? sm.warp[warp][d] : 0u;
-                __syncwarp();
-                if (in && lane == 31 - __clz(peers)) sm.warp[warp][d] = old + __popc(peers);
-                __syncwarp();
-                at[k] = old + __popc(peers & ((1u << lane) - 1u));
-            }
-            __syncthreads();
-            if (tid < bins) {  // the warps' counts -> where each warp's keys of this digit go
-                uint32_t run = sm.base[tid];
-                for (int w = 0; w < SORT_T / 32; ++w) {
-                    const uint32_t c = sm.warp[w][tid];
-                    sm.warp[w][tid] = run;
-                    run += c;
-                }
-                sm.base[tid] = run;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < ITEMS; ++k)
-                if (w0 + k * 32 + lane < i1)
-                    dst[sm.warp[warp][(kv[k].x >> shift) & (uint32_t)(bins - 1)] + at[k]] = kv[k];
-            __syncthreads();
         }
         cluster_sync();  // the pass's list is complete, and the counts have been read
     }
 }
 
+__device__ void fill_absent(const SortArgs& p, FillSmem& sm, uint32_t cluster, uint32_t clusters) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    const uint32_t rank = cluster_ctarank(), blocks = clusters * CL, me = cluster * CL + rank;
+    // Rows in groups of 2^gs, dealt to the blocks in turn: frequent tokens have
+    // low numbers, so ranges of neighbouring rows would leave some blocks
+    // without work (600 MB of zeros in 140 us instead of 100).
+    const int gs = p.group_shift;
+    const int64_t span = (int64_t)blocks * ZROWS;  // rows whose marks fit at once
+    // the lanes that share a row
+    const int units = p.vec ? p.D / 4 : p.D;
+    int g = 1;
+    while (g < 32 && g < units) g <<= 1;
+    for (int64_t lo = 0; lo < p.rows; lo += span) {
+        const uint32_t rows = (uint32_t)min(span, p.rows - lo);
+        const uint32_t groups = (rows + (1u << gs) - 1) >> gs;
+        const uint32_t per = ((groups + blocks - 1) / blocks) << gs;  // marks a block
+        for (uint32_t w = tid; w * 32 < per; w += SORT_T) sm.marks[w] = 0;
+        cluster_sync();
+        for (int64_t i0 = (int64_t)rank * SORT_T + tid; i0 < p.n; i0 += CL * SORT_T * 4) {
+            int64_t t[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int64_t i = i0 + (int64_t)k * CL * SORT_T;
+                t[k] = i < p.n ? p.tok.get(i) - lo : -1;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (t[k] < 0 || t[k] >= (int64_t)rows) continue;
+                const uint32_t group = (uint32_t)t[k] >> gs, turn = group / blocks, owner = group - turn * blocks;
+                if (owner / CL != cluster) continue;
+                const uint32_t at = (turn << gs) | ((uint32_t)t[k] & ((1u << gs) - 1u));
+                asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(
+                                 cluster_addr(&sm.marks[at >> 5], owner % CL)),
+                             "r"(1u << (at & 31))
+                             : "memory");
+            }
+        }
+        cluster_sync();
+        for (uint32_t q = tid / g; q < per; q += SORT_T / g) {
+            if ((sm.marks[q >> 5] >> (q & 31)) & 1u) continue;
+            const uint32_t v = ((((q >> gs) * blocks) + me) << gs) | (q & ((1u << gs) - 1u));
+            if (v >= rows) continue;
+            float* row = p.dw + (lo + v) * p.D;
+            if (p.vec) {
+                for (int j = lane & (g - 1); j < units; j += g)
+                    __stcs(reinterpret_cast<float4*>(row) + j, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+            } else {
+                for (int j = lane & (g - 1); j < units; j += g) __stcs(row + j, 0.0f);
+            }
+        }
+        cluster_sync();  // before the marks are cleared again
+    }
+}
+
+__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(SORT_T) embed_sort_kernel(SortArgs p) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    const int cluster = (int)blockIdx.x / CL, clusters = (int)gridDim.x / CL;
+    if (cluster == 0)
+        sort_positions(p, *reinterpret_cast<SortSmem*>(raw));
+    else
+        fill_absent(p, *reinterpret_cast<FillSmem*>(raw), (uint32_t)(cluster - 1), (uint32_t)(clusters - 1));
+}
+
 // ---- the sums of runs -------------------------------------------------------------------
 
-constexpr int CH = 32;  // sorted positions a chunk
-constexpr int AHEAD = 8;
+constexpr int AHEAD = 8;  // rows whose loads a warp has in flight
 
 struct SumArgs {
     const uint2* list;  // (token, position) by token
     const float* g;
     Rows gm;
     float* dw;
-    float* part;  // [chunks][2][D]: 0: a run that began before the chunk, 1: one that goes on behind it
+    float* part;    // [chunks][2][D]: 0: a run that began before the chunk, 1: one that goes on behind it
+    int* crossing;  // count, then the chunks whose last run begins there and goes on
     int64_t rows;
     int n, D;
+    int ch;  // sorted positions a chunk, at most 32
     int accumulate;
     float scale;
 };
@@ -221,88 +343,154 @@ __device__ __forceinline__ void write_row(const SumArgs& p, int64_t row, int j, 
     store_vec<VEC>(o, a);
 }
 
-// A warp takes one chunk and 32 * VEC columns.
-template <int VEC>
+// A warp takes one chunk and 32 * VEC * VPT columns.  Lane i holds the i-th
+// position's key and row; where runs end is one mask.
+template <int VEC, int VPT>
 __global__ void __launch_bounds__(256) embed_sum_kernel(SumArgs p, int64_t units, int slices) {
     const int lane = threadIdx.x & 31;
     const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (u >= units) return;
-    const int chunk = (int)(u / slices);
-    const int j = (int)(u - (int64_t)chunk * slices) * (32 * VEC) + lane * VEC;
-    const int p0 = chunk * CH, cnt = min(CH, p.n - p0);
+    const int chunk = (int)(u / slices), slice = (int)(u - (int64_t)chunk * slices);
+    const int j0 = slice * (32 * VEC * VPT) + lane * VEC;
+    const int p0 = chunk * p.ch, cnt = min(p.ch, p.n - p0);
     const uint32_t none = (uint32_t)p.rows;
     const uint2 mine = lane < cnt ? p.list[p0 + lane] : make_uint2(none, 0u);
     const uint32_t prev = p0 > 0 ? p.list[p0 - 1].x : none, next = p0 + cnt < p.n ? p.list[p0 + cnt].x : none;
-    const bool in = j < p.D;
-    float a[VEC];
+    const int valid = __popc(__ballot_sync(0xffffffffu, mine.x != none));  // keys that are none come last
+    if (valid == 0) return;
+    const int64_t row = p.gm.offset(mine.y);
+    const uint32_t after = __shfl_down_sync(0xffffffffu, mine.x, 1);
+    const uint32_t ends = __ballot_sync(0xffffffffu, lane < valid && (lane == valid - 1 || after != mine.x));
+    const bool on = valid == cnt && __shfl_sync(0xffffffffu, mine.x, valid - 1) == next;
+    bool before = __shfl_sync(0xffffffffu, mine.x, 0) == prev;
+    float a[VPT][VEC];
 #pragma unroll
-    for (int c = 0; c < VEC; ++c) a[c] = 0.0f;
-    bool first = true;  // the run being summed is the chunk's first
-    for (int i0 = 0; i0 < cnt; i0 += AHEAD) {
-        float v[AHEAD][VEC];
+    for (int q = 0; q < VPT; ++q)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) a[q][c] = 0.0f;
+    for (int i0 = 0; i0 < valid; i0 += AHEAD) {
+        float v[AHEAD][VPT][VEC];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-            const uint32_t key = __shfl_sync(0xffffffffu, mine.x, (i0 + k) & 31);
-            const uint32_t pos = __shfl_sync(0xffffffffu, mine.y, (i0 + k) & 31);
-            if (in && i0 + k < cnt && key != none) {
-                load_once<VEC>(p.g + p.gm.offset(pos) + j, v[k]);
-            } else {
+            const float* g = p.g + __shfl_sync(0xffffffffu, row, (i0 + k) & 31) + j0;
+            if (i0 + k < valid) {
 #pragma unroll
-                for (int c = 0; c < VEC; ++c) v[k][c] = 0.0f;
+                for (int q = 0; q < VPT; ++q)
+                    if (j0 + q * 32 * VEC < p.D) load_once<VEC>(g + q * 32 * VEC, v[k][q]);
             }
         }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             const int i = i0 + k;
-            const uint32_t key = __shfl_sync(0xffffffffu, mine.x, i & 31);
-            const uint32_t after = i + 1 < cnt ? __shfl_sync(0xffffffffu, mine.x, (i + 1) & 31) : next;
-            if (i >= cnt || key == none) return;  // only keys that are none follow
+            if (i >= valid) break;
 #pragma unroll
-            for (int c = 0; c < VEC; ++c) a[c] += v[k][c];
-            if (after == key && i + 1 < cnt) continue;
-            const bool before = first && prev == key, on = after == key;
-            if (in) {
-                if (!before && !on) {
-                    write_row<VEC>(p, key, j, a);
-                } else {
-                    store_vec<VEC>(p.part + ((int64_t)chunk * 2 + (before ? 0 : 1)) * p.D + j, a);
+            for (int q = 0; q < VPT; ++q)
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) a[q][c] += v[k][q][c];
+            if (!((ends >> i) & 1u)) continue;
+            const uint32_t key = __shfl_sync(0xffffffffu, mine.x, i);
+            const bool goes_on = on && i == valid - 1;
+#pragma unroll
+            for (int q = 0; q < VPT; ++q) {
+                const int j = j0 + q * 32 * VEC;
+                if (j < p.D) {
+                    if (!before && !goes_on)
+                        write_row<VEC>(p, key, j, a[q]);
+                    else
+                        store_vec<VEC>(p.part + ((int64_t)chunk * 2 + (before ? 0 : 1)) * p.D + j, a[q]);
                 }
-            }
 #pragma unroll
-            for (int c = 0; c < VEC; ++c) a[c] = 0.0f;
-            first = false;
+                for (int c = 0; c < VEC; ++c) a[q][c] = 0.0f;
+            }
+            // the order of this list does not matter: each entry is summed by itself
+            if (goes_on && !before && slice == 0 && lane == 0) p.crossing[1 + atomicAdd(p.crossing, 1)] = chunk;
+            before = false;
         }
     }
 }
 
-// A run that crosses chunks: its first chunk's part 1, then part 0 of the
-// chunks behind it, in their order.
+// The sum of `count` parts 0 from chunk `c` on, in their order.
 template <int VEC>
-__global__ void __launch_bounds__(256) embed_join_kernel(SumArgs p, int64_t units, int slices) {
-    const int lane = threadIdx.x & 31;
-    const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (u >= units) return;
-    const int chunk = (int)(u / slices);
-    const int j = (int)(u - (int64_t)chunk * slices) * (32 * VEC) + lane * VEC;
-    const int end = (chunk + 1) * CH;  // first position behind the chunk
-    if (end >= p.n) return;
-    const uint32_t key = p.list[end - 1].x;
-    if (key == (uint32_t)p.rows || p.list[end].x != key) return;
-    // does the run begin in this chunk?
-    if (p.list[chunk * CH].x == key && chunk > 0 && p.list[chunk * CH - 1].x == key) return;
-    float a[VEC];
-    if (j < p.D) load_vec<VEC>(p.part + ((int64_t)chunk * 2 + 1) * p.D + j, a);
-    for (int c = chunk + 1;; ++c) {
-        float v[VEC];
-        if (j < p.D) {
-            load_vec<VEC>(p.part + (int64_t)c * 2 * p.D + j, v);
+__device__ __forceinline__ void add_parts(const SumArgs& p, int c, int count, int j, float (&a)[VEC]) {
+    constexpr int U = 8;
+    for (int q = 0; q < count; q += U) {
+        float v[U][VEC];
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) a[q] += v[q];
-        }
-        const int64_t behind = (int64_t)(c + 1) * CH;
-        if (behind >= p.n || p.list[behind].x != key) break;
+        for (int k = 0; k < U; ++k)
+            if (q + k < count) load_vec<VEC>(p.part + (int64_t)(c + q + k) * 2 * p.D + j, v[k]);
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+            if (q + k < count)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) a[e] += v[k][e];
     }
-    if (j < p.D) write_row<VEC>(p, key, j, a);
+}
+
+// A run that crosses chunks: its first chunk's part 1, then part 0 of the
+// chunks behind it, in their order.  A warp takes a run and 32 * VEC columns;
+// runs of more than LONG chunks (one token in thousands of positions) are
+// shared by the block's warps, an eighth of the chunks each.
+constexpr int LONG = 16;
+template <int VEC>
+__global__ void __launch_bounds__(256) embed_join_kernel(SumArgs p, int slices) {
+    __shared__ int long_chunk[8], long_slice[8], long_count[8];
+    __shared__ float eighth[8][32 * VEC];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int runs = *p.crossing;
+    const int64_t units = (int64_t)runs * slices;
+    for (int64_t u0 = (int64_t)blockIdx.x * 8; u0 < units; u0 += (int64_t)gridDim.x * 8) {
+        const int64_t u = u0 + warp;
+        int count = 0;  // chunks behind the first
+        if (u < units) {
+            // neighbouring warps take different runs: the slices of a long one go to different blocks
+            const int slice = (int)(u / runs), chunk = p.crossing[1 + (int)(u - (int64_t)slice * runs)];
+            const int j = slice * (32 * VEC) + lane * VEC;
+            const uint32_t key = p.list[(int64_t)(chunk + 1) * p.ch - 1].x;
+            for (;;) {  // does the run reach into chunk + 1 + count + lane?
+                const int64_t begin = (int64_t)(chunk + 1 + count + lane) * p.ch;
+                const uint32_t go = __ballot_sync(0xffffffffu, begin < p.n && p.list[begin < p.n ? begin : 0].x == key);
+                const int full = go == 0xffffffffu ? 32 : __ffs(~go) - 1;
+                count += full;
+                if (full < 32) break;
+            }
+            if (count <= LONG && j < p.D) {
+                float a[VEC];
+                load_vec<VEC>(p.part + ((int64_t)chunk * 2 + 1) * p.D + j, a);
+                add_parts<VEC>(p, chunk + 1, count, j, a);
+                write_row<VEC>(p, key, j, a);
+            }
+            if (lane == 0) long_chunk[warp] = chunk, long_slice[warp] = slice;
+        }
+        if (lane == 0) long_count[warp] = count > LONG ? count : 0;
+        __syncthreads();
+        for (int q = 0; q < 8; ++q) {
+            const int n = long_count[q];
+            if (n == 0) continue;
+            const int chunk = long_chunk[q], j = long_slice[q] * (32 * VEC) + lane * VEC;
+            const int per = (n + 7) / 8, c0 = min(n, warp * per), c1 = min(n, c0 + per);
+            float a[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) a[e] = 0.0f;
+            if (j < p.D) {
+                if (warp == 0) load_vec<VEC>(p.part + ((int64_t)chunk * 2 + 1) * p.D + j, a);
+                add_parts<VEC>(p, chunk + 1 + c0, c1 - c0, j, a);
+            }
+            store_vec<VEC>(&eighth[warp][lane * VEC], a);
+            __syncthreads();
+            if (warp == 0 && j < p.D) {
+#pragma unroll
+                for (int w = 1; w < 8; ++w) {
+                    float v[VEC];
+                    load_vec<VEC>(&eighth[w][lane * VEC], v);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) a[e] += v[e];
+                }
+                write_row<VEC>(p, p.list[(int64_t)(chunk + 1) * p.ch - 1].x, j, a);
+            }
+            __syncthreads();
+        }
+        __syncthreads();  // the lists are written again
+    }
 }
 
 int table_view(const tlc_tensor* w, const char* op, const char* name, RowView& v) {
@@ -337,18 +525,45 @@ int launch_embed(const EmbFwd& p, cudaStream_t s) {
     return check_launch(kFwd);
 }
 
-template <int VEC>
+template <int VEC, int VPT>
 int launch_sums(const SumArgs& p, cudaStream_t s) {
-    const int slices = (p.D + 32 * VEC - 1) / (32 * VEC);
-    const int64_t units = (int64_t)((p.n + CH - 1) / CH) * slices;
-    const int64_t blocks = (units + 7) / 8;
+    const int64_t chunks = (p.n + p.ch - 1) / p.ch;
+    const int slices = (p.D + 32 * VEC * VPT - 1) / (32 * VEC * VPT);
+    const int64_t blocks = (chunks * slices + 7) / 8;
     if (blocks > INT32_MAX) return set_error(TLC_ERR_UNSUPPORTED, "embedding_backward: too many tokens");
-    embed_sum_kernel<VEC><<<(unsigned)blocks, 256, 0, s>>>(p, units, slices);
+    embed_sum_kernel<VEC, VPT><<<(unsigned)blocks, 256, 0, s>>>(p, chunks * slices, slices);
     count_launch();
     TLC_TRY(check_launch(kBwd));
-    embed_join_kernel<VEC><<<(unsigned)blocks, 256, 0, s>>>(p, units, slices);
+    if (chunks == 1) return TLC_OK;  // no run crosses
+    // the number of crossing runs is on the device: enough blocks to keep every SM busy
+    const int thin = (p.D + 32 * VEC - 1) / (32 * VEC);
+    embed_join_kernel<VEC><<<(unsigned)std::min<int64_t>((chunks * thin + 7) / 8, 148 * 4), 256, 0, s>>>(p, thin);
     count_launch();
     return check_launch(kBwd);
+}
+
+// The most clusters of the sort kernel that run at once on the current device.
+int max_clusters(int* out) {
+    static DeviceOnce once;
+    static int clusters[64];
+    int dev = 0;
+    TLC_TRY(device_once(
+        once,
+        [](int d) -> int {
+            const int smem = (int)std::max(sizeof(SortSmem), sizeof(FillSmem));
+            TLC_CUDA_TRY(cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(CL);
+            cfg.blockDim = dim3(SORT_T);
+            cfg.dynamicSmemBytes = (size_t)smem;
+            int n = 0;
+            TLC_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, embed_sort_kernel, &cfg));
+            clusters[d] = std::max(n, 2);
+            return TLC_OK;
+        },
+        &dev));
+    *out = clusters[dev];
+    return TLC_OK;
 }
 
 }  // namespace
@@ -405,11 +620,20 @@ extern "C" int tlc_embedding_backward(const tlc_tensor* grad, const tlc_index* t
     TLC_TRY(no_overlap(kBwd, "dweight", ed, "tokens", et));
     if (n > INT32_MAX - TILE) return set_error(TLC_ERR_UNSUPPORTED, "embedding_backward: too many tokens");
     if (vd.numel == 0) return TLC_OK;
-    if (!accumulate) TLC_TRY(launch_fill_zero(dweight->data, vd.numel, s));
-    if (n == 0) return TLC_OK;
-    RowScratch cg(s), cl(s), cp(s);
+    if (n == 0) return accumulate ? TLC_OK : launch_fill_zero(dweight->data, vd.numel, s);
+    RowScratch cg(s), cw(s);
     TLC_TRY(unit_rows(grad, vg, cg));
-    TLC_TRY(scratch_alloc(&cl.p, sizeof(uint2) * 2 * (size_t)n, s));
+    const int D = (int)vd.cols;
+    const bool vec = D % 4 == 0 && vg.map.multiple_of(4) && aligned_to(vg.data, 16) && aligned_to(dweight->data, 16);
+    // 32 positions a chunk; 16 where that would leave an SM fewer than 16 warps
+    const int64_t slices = (D + 255) / 256;
+    const int ch = (n / 32) * slices >= 148 * 16 ? 32 : 16;
+    const int64_t chunks = (n + ch - 1) / ch;
+    // one workspace: the parts, the two lists, the crossing runs
+    const size_t part_bytes = sizeof(float) * 2 * (size_t)chunks * (size_t)D;
+    const size_t list_at = (part_bytes + 15) & ~size_t(15), list_bytes = sizeof(uint2) * (size_t)n;
+    TLC_TRY(scratch_alloc(&cw.p, list_at + 2 * list_bytes + sizeof(int) * (size_t)(chunks + 1), s));
+    char* ws = static_cast<char*>(cw.p);
     SortArgs q{};
     q.tok = tok;
     q.rows = vd.rows;
@@ -418,11 +642,21 @@ extern "C" int tlc_embedding_backward(const tlc_tensor* grad, const tlc_index* t
     while ((vd.rows >> width) != 0) ++width;
     q.passes = (width + MAX_BITS - 1) / MAX_BITS;
     q.bits = (width + q.passes - 1) / q.passes;
-    q.a = static_cast<uint2*>(cl.p);
+    q.a = reinterpret_cast<uint2*>(ws + list_at);
     q.b = q.a + n;
-    static DeviceOnce once;
-    TLC_TRY(smem_limit_once(once, embed_sort_kernel, (int)sizeof(SortSmem)));
-    embed_sort_kernel<<<CL, SORT_T, sizeof(SortSmem), s>>>(q);
+    q.crossing = reinterpret_cast<int*>(q.b + n);
+    int clusters = 1;
+    if (!accumulate) {
+        TLC_TRY(max_clusters(&clusters));
+        q.dw = dweight->data;
+        q.D = D;
+        q.vec = D % 4 == 0 && aligned_to(q.dw, 16);
+        while (q.group_shift < 5 && ((int64_t)D * 4 << q.group_shift) < 2048) ++q.group_shift;
+    } else {
+        int unused;
+        TLC_TRY(max_clusters(&unused));  // sets the kernel's shared-memory limit
+    }
+    embed_sort_kernel<<<CL * clusters, SORT_T, std::max(sizeof(SortSmem), sizeof(FillSmem)), s>>>(q);
     count_launch();
     TLC_TRY(check_launch(kBwd));
     SumArgs p{};
@@ -430,14 +664,13 @@ extern "C" int tlc_embedding_backward(const tlc_tensor* grad, const tlc_index* t
     p.g = vg.data;
     p.gm = vg.map;
     p.dw = dweight->data;
+    p.part = reinterpret_cast<float*>(ws);
+    p.crossing = q.crossing;
     p.rows = vd.rows;
     p.n = (int)n;
-    p.D = (int)vd.cols;
+    p.D = D;
     p.accumulate = accumulate != 0;
     p.scale = scale;
-    const int64_t chunks = (n + CH - 1) / CH;
-    TLC_TRY(scratch_alloc(&cp.p, sizeof(float) * 2 * (size_t)chunks * (size_t)p.D, s));
-    p.part = cp.f();
-    const bool vec = p.D % 4 == 0 && vg.map.multiple_of(4) && aligned_to(p.g, 16) && aligned_to(p.dw, 16);
-    return vec ? launch_sums<4>(p, s) : launch_sums<1>(p, s);
+    p.ch = ch;
+    return vec ? launch_sums<4, 2>(p, s) : launch_sums<1, 4>(p, s);
 }
