@@ -32,32 +32,31 @@ struct EmbFwd {
     float scale;
 };
 
-// A warp copies 4 vectors a lane of one row.
+// A warp copies EV vectors a lane of one row.  Rows and results are read and
+// written once: streaming loads and stores leave the L2 to the other tensors.
+constexpr int EV = 4;
 template <int VEC>
 __global__ void __launch_bounds__(256) embed_kernel(EmbFwd p, int pieces) {
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * 8;
     for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < p.n * pieces; u += warps) {
         const int64_t i = u / pieces;
-        const int j0 = (int)(u - i * pieces) * (128 * VEC) + lane * VEC;
+        const int j0 = (int)(u - i * pieces) * (32 * EV * VEC) + lane * VEC;
         const int64_t t = p.tok.get(i);
         const bool ok = t >= 0 && t < p.rows;
         const float fill = t == -1 ? 0.0f : __int_as_float(0x7fc00000);
-        const float* src = p.w + (ok ? t : 0) * p.w_rs;
-        float v[4][VEC];
+        const float* src = p.w + (ok ? t : 0) * p.w_rs + j0;
+        float v[EV][VEC];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int j = j0 + k * 32 * VEC;
-            if (ok && j < p.D) load_vec<VEC>(src + j, v[k]);
-        }
-        float* dst = p.out + i * p.D;
+        for (int k = 0; k < EV; ++k)
+            if (ok && j0 + k * 32 * VEC < p.D) load_once<VEC>(src + k * 32 * VEC, v[k]);
+        float* dst = p.out + i * p.D + j0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int j = j0 + k * 32 * VEC;
-            if (j < p.D) {
+        for (int k = 0; k < EV; ++k) {
+            if (j0 + k * 32 * VEC < p.D) {
 #pragma unroll
                 for (int c = 0; c < VEC; ++c) v[k][c] = ok ? v[k][c] * p.scale : fill;
-                store_vec<VEC>(dst + j, v[k]);
+                store_once<VEC>(dst + k * 32 * VEC, v[k]);
             }
         }
     }
@@ -518,7 +517,7 @@ int check_scale(float scale, const char* op) {
 
 template <int VEC>
 int launch_embed(const EmbFwd& p, cudaStream_t s) {
-    const int pieces = (p.D + 128 * VEC - 1) / (128 * VEC);
+    const int pieces = (p.D + 32 * EV * VEC - 1) / (32 * EV * VEC);
     const int64_t want = (p.n * pieces + 7) / 8;
     embed_kernel<VEC><<<(unsigned)std::min<int64_t>(want, INT32_MAX), 256, 0, s>>>(p, pieces);
     count_launch();

@@ -358,14 +358,6 @@ __global__ void __launch_bounds__(512) ln_bwd_finish_kernel(const float* __restr
     }
 }
 
-int sm_count() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
-        return 148;
-    return sms;
-}
-
 constexpr const char* kFwd = "layer_norm";
 constexpr const char* kBwd = "layer_norm_backward";
 

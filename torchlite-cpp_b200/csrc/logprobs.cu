@@ -55,6 +55,32 @@ constexpr float kFloor = -160.0f;
 
 // ---- running sums ---------------------------------------------------------------------
 
+// Two floats in one 64-bit register pair: one instruction for both.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ void unpair(Pair p, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
 // m: maximum (-inf: nothing yet), l = sum 2^y, w = sum 2^y y with y = a (x - m), a = scale log2 e.
 struct Run {
     float m = -INFINITY, l = 0.0f, w = 0.0f;
@@ -80,21 +106,56 @@ struct Run {
     }
 };
 
-template <int N>
-__device__ __forceinline__ void run_add(Run& r, const float (&v)[N], float a) {
-    float top = v[0];
+// Adds values to a run, two at a time: 9 instructions for two values.
+struct PairRun {
+    float m = -INFINITY;
+    float rest = -INFINITY;  // the maximum of the batches other than number `where`, which has m
+    int where = 0;
+    Pair l, w, a2;
+    float a;
+    __device__ __forceinline__ explicit PairRun(float scale2) : l(0), w(0), a2(pair(scale2, scale2)), a(scale2) {}
+    template <int N>
+    __device__ __forceinline__ void add(const float (&v)[N], int batch) {
+        float top = v[0];
 #pragma unroll
-    for (int i = 1; i < N; ++i) top = max_nan(top, v[i]);
-    if (!(top <= r.m)) r.raise(max_nan(top, r.m), a);  // also when top is NaN
-    const float m = r.m == -INFINITY ? 0.0f : r.m;
+        for (int i = 1; i < N; ++i) top = max_nan(top, v[i]);
+        if (!(top <= m)) {  // also when top is NaN
+            const float to = max_nan(top, m);
+            if (m != -INFINITY) {
+                const float y = max_nan((m - to) * a, kFloor), c = ex2(y);
+                w = mul2(pair(c, c), fma2(pair(y, y), l, w));
+                l = mul2(pair(c, c), l);
+            }
+            rest = max_nan(rest, m);
+            m = to;
+            where = batch;
+        } else {
+            rest = max_nan(rest, top);
+        }
+        const float base = m == -INFINITY ? 0.0f : -m;
+        const Pair shift = pair(base, base);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float y = max_nan((v[i] - m) * a, kFloor);
-        const float e = ex2(y);
-        r.l += e;
-        r.w = fmaf(e, y, r.w);
+        for (int i = 0; i < N; i += 2) {
+            const Pair y2 = mul2(add2(pair(v[i], i + 1 < N ? v[i + 1] : -INFINITY), shift), a2);
+            float y0, y1;
+            unpair(y2, y0, y1);
+            y0 = max_nan(y0, kFloor), y1 = max_nan(y1, kFloor);
+            const Pair e = pair(ex2(y0), ex2(y1));
+            l = add2(l, e);
+            w = fma2(e, pair(y0, y1), w);
+        }
     }
-}
+    __device__ __forceinline__ Run sum() const {
+        Run r;
+        float x, y;
+        r.m = m;
+        unpair(l, x, y);
+        r.l = x + y;
+        unpair(w, x, y);
+        r.w = x + y;
+        return r;
+    }
+};
 
 __device__ __forceinline__ Run warp_run(Run r, float a) {
 #pragma unroll
@@ -120,6 +181,10 @@ __device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
     return ((uint64_t)order_of(v) << 32) | (uint32_t)~index;
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)key; }
+__device__ __forceinline__ float value_of(uint64_t key) {
+    const uint32_t u = (uint32_t)(key >> 32);
+    return u == 0xffffffffu ? __int_as_float(0x7fc00000) : __uint_as_float((u & 0x80000000u) ? u ^ 0x80000000u : ~u);
+}
 
 struct LpFwd {
     const float* x;
@@ -135,8 +200,19 @@ struct LpFwd {
     int top_wide;
 };
 
+// The token of a row and its logit.
+struct Asked {
+    int64_t t = -1;
+    float x = 0.0f;
+    __device__ __forceinline__ Asked(const LpFwd& p, int64_t r, const float* row) {
+        if (!p.logp) return;
+        t = p.tok.get(r);
+        if (t >= 0 && t < p.V) x = row[t];
+    }
+};
+
 // What the row's results are, from its sums.
-__device__ __forceinline__ void row_results(const LpFwd& p, int64_t r, const float* x, const Run& s) {
+__device__ __forceinline__ void row_results(const LpFwd& p, int64_t r, const Asked& q, const Run& s) {
     const bool none = s.m == -INFINITY;
     const float log_l = none ? 0.0f : logf(s.l);
     if (p.stats) {
@@ -145,22 +221,20 @@ __device__ __forceinline__ void row_results(const LpFwd& p, int64_t r, const flo
     }
     if (p.entropy) p.entropy[r] = none ? 0.0f : fmaxf(log_l - kLn2 * (s.w / s.l), 0.0f) + (s.l != s.l ? s.l : 0.0f);
     if (p.logp) {
-        const int64_t t = p.tok.get(r);
         float lp = 0.0f;
-        if (t != -1) {
-            if (t < 0 || t >= p.V)
+        if (q.t != -1) {
+            if (q.t < 0 || q.t >= p.V)
                 lp = __int_as_float(0x7fc00000);
             else
-                lp = none ? -INFINITY : (x[t] - s.m) * p.scale - log_l;
+                lp = none ? -INFINITY : (q.x - s.m) * p.scale - log_l;
         }
         p.logp[r] = lp;
     }
 }
 
-__device__ __forceinline__ void top_result(const LpFwd& p, int64_t r, const float* x, int i, uint64_t key, float m,
-                                           float log_l) {
+__device__ __forceinline__ void top_result(const LpFwd& p, int64_t r, int i, uint64_t key, float m, float log_l) {
     const uint32_t j = index_of(key);
-    p.top_logp[r * p.top + i] = m == -INFINITY ? -INFINITY : (x[j] - m) * p.scale - log_l;
+    p.top_logp[r * p.top + i] = m == -INFINITY ? -INFINITY : (value_of(key) - m) * p.scale - log_l;
     if (p.top_wide)
         static_cast<int64_t*>(p.top_tok)[r * p.top + i] = j;
     else
@@ -178,11 +252,10 @@ __global__ void __launch_bounds__(256) lp_warp_kernel(LpFwd p) {
         float v[VPT];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) v[i] = 32 * i + lane < p.V ? __ldcs(x + 32 * i + lane) : -INFINITY;
-        Run s;
-        run_add(s, v, p.a);
-        s = warp_run(s, p.a);
-        // a lane without values of its own still counted -inf: nothing
-        if (lane == 0) row_results(p, r, x, s);
+        PairRun own(p.a);
+        own.add(v, 0);  // a lane without values of its own counts -inf: nothing
+        const Run s = warp_run(own.sum(), p.a);
+        if (lane == 0) row_results(p, r, Asked(p, r, x), s);
         if (p.top) {
             const float log_l = s.m == -INFINITY ? 0.0f : logf(s.l);
             uint64_t last = ~0ull;  // the key picked before
@@ -200,7 +273,7 @@ __global__ void __launch_bounds__(256) lp_warp_kernel(LpFwd p) {
                 const uint32_t lo =
                     __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
                 last = ((uint64_t)hi << 32) | lo;
-                if (lane == 0) top_result(p, r, x, i, last, s.m, log_l);
+                if (lane == 0) top_result(p, r, i, last, s.m, log_l);
             }
         }
     }
@@ -209,6 +282,8 @@ __global__ void __launch_bounds__(256) lp_warp_kernel(LpFwd p) {
 // ---- a row for a block or a cluster of blocks ----------------------------------------------
 
 constexpr int CAP = 512;  // candidates for the alternatives that a block keeps
+constexpr int BATCH = 4;  // float4 that a thread takes at once
+constexpr int STAGES = 3;  // batches in shared memory or on their way to it
 
 template <int T>
 struct LpSmem {
@@ -218,9 +293,10 @@ struct LpSmem {
     uint32_t bound;
     int threads, found;
     uint16_t look[T];                  // threads whose values reach the bound
+    int16_t batch[T];                  // and in which batch: a number, -1 (the single value), -2 (any)
     uint64_t cand[CAP];
     uint64_t best[kMaxTop];            // the block's alternatives, in order
-    uint64_t all[16 * kMaxTop];        // the cluster's, in its first block
+    uint64_t all[8 * kMaxTop];         // the cluster's, in its first block
     uint32_t hist[256];
     int bin, need;
 };
@@ -251,9 +327,10 @@ struct Part {
 };
 
 // The part's `k` largest keys in order, into sm.best (k <= part.n values; the
-// rest of sm.best is 0).  top: the largest value of this thread (-inf: none).
+// rest of sm.best is 0).  top: the largest value of this thread (-inf: none),
+// which its batch `where` has (-1: its single value), rest: of its others.
 template <int T>
-__device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top) {
+__device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top, float rest, int where) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int G = T / 64;  // neighbouring lanes a group
     uint32_t g = order_of(top);
@@ -274,7 +351,12 @@ __device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top) {
     }
     __syncthreads();
     const uint32_t bound = sm.bound;
-    if (order_of(top) >= bound) sm.look[atomicAdd(&sm.threads, 1)] = (uint16_t)tid;
+    // mostly no other batch of the thread reaches the bound: then one is looked at, else all
+    if (order_of(top) >= bound) {
+        const int c = atomicAdd(&sm.threads, 1);
+        sm.look[c] = (uint16_t)tid;
+        sm.batch[c] = (int16_t)(order_of(rest) >= bound ? -2 : where);
+    }
     __syncthreads();
     const int threads = sm.threads;
     auto take = [&](float v, int at) {
@@ -284,8 +366,10 @@ __device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top) {
         }
     };
     for (int q = warp; q < threads; q += T / 32) {
-        const int t = sm.look[q];
-        for (int i = t + T * lane; i < part.vecs; i += T * 32) {
+        const int t = sm.look[q], only = sm.batch[q];
+        const int begin = only == -2 ? 0 : only == -1 ? part.vecs : only * BATCH * T;
+        const int end = only == -2 ? part.vecs : only == -1 ? 0 : min(part.vecs, begin + BATCH * T);
+        for (int i = begin + t + T * lane; i < end; i += T * 32) {
             const float4 f = part.vec(i);
             const int at = part.head + 4 * i;
             take(f.x, at);
@@ -293,7 +377,7 @@ __device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top) {
             take(f.z, at + 2);
             take(f.w, at + 3);
         }
-        if (lane == 0) {
+        if (lane == 0 && only < 0) {
             const int at = part.single(t);
             if (at >= 0) take(part.x[at], at);
         }
@@ -352,100 +436,141 @@ __device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top) {
     __syncthreads();
 }
 
-// C blocks a row (1, or the cluster's size), T threads a block.
+// C blocks a row (1, or the cluster's size), T threads a block, each block (or
+// cluster) with several rows.  The rows' values come through a ring of
+// asynchronous copies that runs across the rows' ends, so that the memory stays
+// busy while a row's results are put together; a thread copies what it reads
+// itself, which needs no barrier.
 template <int T>
 __global__ void __launch_bounds__(T) lp_row_kernel(LpFwd p, int C) {
+    extern __shared__ __align__(16) float4 ring[];  // [STAGES][BATCH][T]
     __shared__ LpSmem<T> sm;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = C > 1 ? (int)cluster_ctarank() : 0;
-    const int64_t r = blockIdx.x / C;
-    const float* x = p.x + p.xm.offset(r);
+    const int64_t first = blockIdx.x / C, step = gridDim.x / C;
     const int per = ((p.V + C - 1) / C + 31) & ~31;
     const int lo = (int)min((int64_t)p.V, (int64_t)rank * per), hi = (int)min((int64_t)p.V, (int64_t)lo + per);
-    const Part part(x, lo, hi);
-    Run s;
-    constexpr int U = 4;
-    int i = tid;
-    for (; i + (U - 1) * T < part.vecs; i += U * T) {
-        float v[4 * U];
+
+    int64_t ahead_row = first;  // the next batch to copy
+    int ahead_at = 0;
+    Part ahead(p.x + p.xm.offset(first), lo, hi);
+    auto fetch = [&](int stage) {
+        if (ahead_row < p.rows) {
+            const float4* from = reinterpret_cast<const float4*>(ahead.x + ahead.head);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float4 f = part.vec(i + u * T);
-            v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
+            for (int u = 0; u < BATCH; ++u) {
+                const int i = ahead_at + tid + u * T;
+                if (i < ahead.vecs)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
+                                     __cvta_generic_to_shared(&ring[(stage * BATCH + u) * T + tid]))),
+                                 "l"(from + i)
+                                 : "memory");
+            }
+            ahead_at += BATCH * T;
+            if (ahead_at >= ahead.vecs) {
+                ahead_at = 0;
+                ahead_row += step;
+                if (ahead_row < p.rows) ahead = Part(p.x + p.xm.offset(ahead_row), lo, hi);
+            }
         }
-        run_add(s, v, p.a);
-    }
-    for (; i < part.vecs; i += T) {
-        const float4 f = part.vec(i);
-        const float v[4] = {f.x, f.y, f.z, f.w};
-        run_add(s, v, p.a);
-    }
-    if (const int at = part.single(tid); at >= 0) {
-        const float v[1] = {part.x[at]};
-        run_add(s, v, p.a);
-    }
-    const float top = s.m;
-    s = warp_run(s, p.a);
-    if (lane == 0) sm.m[warp] = s.m, sm.l[warp] = s.l, sm.w[warp] = s.w;
-    __syncthreads();
-    if (warp == 0) {
-        Run q;
-        if (lane < T / 32) q.m = sm.m[lane], q.l = sm.l[lane], q.w = sm.w[lane];
-        q = warp_run(q, p.a);
-        if (lane == 0) sm.row_m = q.m, sm.row_l = q.l, sm.row_w = q.w;
-    }
-    const int k = min(p.top, part.n);
-    if (p.top > 0 && k > 0) part_top(sm, part, k, top);
-    else if (p.top > 0 && tid < kMaxTop) sm.best[tid] = 0;
-    __syncthreads();
-    if (C == 1) {
-        if (tid == 0) {
-            Run q;
-            q.m = sm.row_m, q.l = sm.row_l, q.w = sm.row_w;
-            row_results(p, r, x, q);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int q = 0; q < STAGES; ++q) fetch(q);
+    int stage = 0;
+    for (int64_t r = first; r < p.rows; r += step) {
+        const float* x = p.x + p.xm.offset(r);
+        const Part part(x, lo, hi);
+        const int at = part.single(tid);
+        const float alone = at >= 0 ? part.x[at] : -INFINITY;
+        const bool asks = tid == 0 && rank == 0;
+        const Asked asked = asks ? Asked(p, r, x) : Asked(LpFwd{}, 0, nullptr);
+        PairRun own(p.a);
+        int batch = 0;
+        do {  // one batch even of a row without float4, as fetch() has it
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+            float v[4 * BATCH];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int i = (batch * BATCH + u) * T + tid;
+                float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (i < part.vecs) f = ring[(stage * BATCH + u) * T + tid];
+                v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
+            }
+            fetch(stage);  // into what was just read
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            own.add(v, batch);
+            ++batch;
+        } while (batch * BATCH * T < part.vecs);
+        if (at >= 0) {
+            const float v[1] = {alone};
+            own.add(v, -1);
         }
-        if (tid < p.top) {
-            const float log_l = sm.row_m == -INFINITY ? 0.0f : logf(sm.row_l);
-            top_result(p, r, x, tid, sm.best[tid], sm.row_m, log_l);
-        }
-        return;
-    }
-    cluster_sync();
-    if (rank == 0) {
+        const Run s = warp_run(own.sum(), p.a);
+        if (lane == 0) sm.m[warp] = s.m, sm.l[warp] = s.l, sm.w[warp] = s.w;
+        __syncthreads();
         if (warp == 0) {
             Run q;
-            if (lane < C) {
-                auto get = [&](const float* f) {
-                    float v;
-                    const uint32_t at = mapa(static_cast<uint32_t>(__cvta_generic_to_shared(f)), (uint32_t)lane);
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-                    return v;
-                };
-                q.m = get(&sm.row_m), q.l = get(&sm.row_l), q.w = get(&sm.row_w);
-            }
+            if (lane < T / 32) q.m = sm.m[lane], q.l = sm.l[lane], q.w = sm.w[lane];
             q = warp_run(q, p.a);
-            if (lane == 0) {
-                row_results(p, r, x, q);
-                sm.m[0] = q.m, sm.l[0] = q.l;
+            if (lane == 0) sm.row_m = q.m, sm.row_l = q.l, sm.row_w = q.w;
+        }
+        const int k = min(p.top, part.n);
+        if (k > 0)
+            part_top(sm, part, k, own.m, own.rest, own.where);
+        else if (p.top > 0 && tid < kMaxTop)
+            sm.best[tid] = 0;
+        __syncthreads();
+        if (C == 1) {
+            if (tid == 0) {
+                Run q;
+                q.m = sm.row_m, q.l = sm.row_l, q.w = sm.row_w;
+                row_results(p, r, asked, q);
+            }
+            if (tid < p.top) {
+                const float log_l = sm.row_m == -INFINITY ? 0.0f : logf(sm.row_l);
+                top_result(p, r, tid, sm.best[tid], sm.row_m, log_l);
+            }
+            continue;  // what the next row writes first, nobody reads here
+        }
+        cluster_sync();
+        if (rank == 0) {
+            if (warp == 0) {
+                Run q;
+                if (lane < C) {
+                    auto get = [&](const float* f) {
+                        float v;
+                        const uint32_t a = mapa(static_cast<uint32_t>(__cvta_generic_to_shared(f)), (uint32_t)lane);
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+                        return v;
+                    };
+                    q.m = get(&sm.row_m), q.l = get(&sm.row_l), q.w = get(&sm.row_w);
+                }
+                q = warp_run(q, p.a);
+                if (lane == 0) {
+                    row_results(p, r, asked, q);
+                    sm.m[0] = q.m, sm.l[0] = q.l;
+                }
+            }
+            for (int c = tid; c < C * p.top; c += T) {
+                const int from = c / p.top;
+                const uint32_t a =
+                    mapa(static_cast<uint32_t>(__cvta_generic_to_shared(&sm.best[c - from * p.top])), (uint32_t)from);
+                asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(sm.all[c]) : "r"(a) : "memory");
+            }
+            __syncthreads();
+            const float log_l = sm.m[0] == -INFINITY ? 0.0f : logf(sm.l[0]);
+            for (int c = tid; c < C * p.top; c += T) {
+                const uint64_t key = sm.all[c];
+                if (key == 0) continue;  // a block with fewer values
+                int above = 0;
+                for (int o = 0; o < C * p.top; ++o) above += sm.all[o] > key;
+                if (above < p.top) top_result(p, r, above, key, sm.m[0], log_l);
             }
         }
-        for (int c = tid; c < C * p.top; c += T) {
-            const int from = c / p.top;
-            const uint32_t at =
-                mapa(static_cast<uint32_t>(__cvta_generic_to_shared(&sm.best[c - from * p.top])), (uint32_t)from);
-            asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(sm.all[c]) : "r"(at) : "memory");
-        }
-        __syncthreads();
-        const float log_l = sm.m[0] == -INFINITY ? 0.0f : logf(sm.l[0]);
-        for (int c = tid; c < C * p.top; c += T) {
-            const uint64_t key = sm.all[c];
-            if (key == 0) continue;  // a block with fewer values
-            int above = 0;
-            for (int o = 0; o < C * p.top; ++o) above += sm.all[o] > key;
-            if (above < p.top) top_result(p, r, x, above, key, sm.m[0], log_l);
-        }
+        cluster_sync();  // the first block has read the others' shared memory
     }
-    cluster_sync();  // the first block has read the others' shared memory
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ---- the gradient ---------------------------------------------------------------------------
@@ -460,65 +585,110 @@ struct LpBwd {
     float scale;
 };
 
+// A row's constants: with d = x - m,
+//   p = 2^(d a - log2 l),  log p + H = d scale + (H - log l),
+//   dx = p (g' + h' (log p + H)) and g scale more at the token, g' = -g scale, h' = -h scale.
+// Two roundings of an exponent of size y cost y 2^-24 relative to p each.
 struct RowGrad {
-    float m, log_l, H, g, h, scale;
+    float m, a, scale, log2_l, offset, g, h;
     int64_t t;
     bool none;
     __device__ __forceinline__ RowGrad(const LpBwd& p, int64_t r) {
         const float* st = p.stats + p.sm.offset(r);
-        m = st[0], log_l = st[1];
+        m = st[0];
+        const float log_l = st[1];
         t = p.tok.get(r);
-        g = p.g && t != -1 ? p.g[p.gm.offset(r)] : 0.0f;
+        g = p.g && t != -1 ? -p.scale * p.g[p.gm.offset(r)] : 0.0f;
         if (p.g && (t < -1 || t >= p.V)) g = __int_as_float(0x7fc00000);
-        h = p.h ? p.h[p.hm.offset(r)] : 0.0f;
-        H = p.h ? p.entropy[p.em.offset(r)] : 0.0f;
+        h = p.h ? -p.scale * p.h[p.hm.offset(r)] : 0.0f;
+        offset = p.h ? p.entropy[p.em.offset(r)] - log_l : 0.0f;
         none = m == -INFINITY;
         scale = p.scale;
+        a = p.scale * kLog2e;
+        log2_l = log_l * kLog2e;
     }
-    __device__ __forceinline__ float at(float x, int64_t j) const {
-        if (none) return 0.0f;
-        const float lp = max_nan(fmaf(x - m, scale, -log_l), kFloor);
-        const float pr = expf(lp);  // to 1 ulp: the SMs have time for it beside 8 bytes a value
-        // g (1[j = t] - p) - h p (log p + H)
-        float d = -pr * fmaf(h, lp + H, g);
-        if (j == t) d += g;
-        return d * scale;
+    template <bool ENT>
+    __device__ __forceinline__ float at(float x) const {
+        const float d = x - m;
+        const float pr = ex2(fmaf(d, a, -log2_l));
+        if constexpr (!ENT) return pr * g;
+        // where p is 0 the exponent may be -inf; p is 0 from -104 on
+        return pr * fmaf(h, max_nan(fmaf(d, scale, offset), -1000.0f), g);
     }
 };
 
-// 256 threads for a run of BW values of one row.
-constexpr int BW = 8192;
-template <bool VEC>
+// 256 threads for a run of BW values of one row, all loaded before the first is
+// written.
+constexpr int BW = 16384;
+template <bool VEC, bool ENT>
 __global__ void __launch_bounds__(256) lp_bwd_kernel(LpBwd p, int pieces) {
     const int64_t r = blockIdx.x / pieces;
     const int lo = (int)(blockIdx.x - r * pieces) * BW, hi = min(p.V, lo + BW);
     const float* x = p.x + p.xm.offset(r);
-    float* dx = p.dx + r * p.V;
-    const RowGrad q(p, r);
+    float* d = p.dx + r * p.V + lo;
+    const int n = hi - lo, tid = threadIdx.x;
+    // the values are asked for before the row's constants, which take as long
     if constexpr (VEC) {
         const Part part(x, lo, hi);
-        float* d = dx + lo;
-        for (int i = threadIdx.x; i < part.vecs; i += 256) {
-            const float4 f = *(reinterpret_cast<const float4*>(part.x + part.head) + i);
-            const int64_t j = lo + part.head + 4 * i;
-            float4 y;
-            y.x = q.at(f.x, j), y.y = q.at(f.y, j + 1), y.z = q.at(f.z, j + 2), y.w = q.at(f.w, j + 3);
-            *(reinterpret_cast<float4*>(d + part.head) + i) = y;
+        const float4* from = reinterpret_cast<const float4*>(part.x + part.head);
+        float4* to = reinterpret_cast<float4*>(d + part.head);
+        constexpr int U = BW / 4 / 256;
+        float4 f[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (tid + u * 256 < part.vecs) f[u] = __ldcs(from + tid + u * 256);
+        const int at = part.single(tid);
+        const float alone = at >= 0 ? part.x[at] : 0.0f;
+        const RowGrad q(p, r);
+        const int tok = q.t >= lo && q.t < hi ? (int)(q.t - lo) : -1;  // the token's place here
+        if (at >= 0) d[at] = q.none ? 0.0f : q.at<ENT>(alone) - (at == tok ? q.g : 0.0f);
+        const int tv = tok < part.head ? -1 : (tok - part.head) >> 2;  // the token's vector
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = tid + u * 256;
+            if (i < part.vecs) {
+                float4 y;
+                y.x = q.at<ENT>(f[u].x), y.y = q.at<ENT>(f[u].y), y.z = q.at<ENT>(f[u].z), y.w = q.at<ENT>(f[u].w);
+                if (i == tv) {
+                    const int c = (tok - part.head) & 3;
+                    if (c == 0) y.x -= q.g;
+                    if (c == 1) y.y -= q.g;
+                    if (c == 2) y.z -= q.g;
+                    if (c == 3) y.w -= q.g;
+                }
+                if (q.none) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // no distribution, no gradient
+                __stcs(to + i, y);
+            }
         }
-        if (const int at = part.single(threadIdx.x); at >= 0) d[at] = q.at(part.x[at], lo + at);
     } else {
-        for (int j = lo + threadIdx.x; j < hi; j += 256) dx[j] = q.at(x[j], j);
+        constexpr int U = BW / 256;
+        float f[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (tid + u * 256 < n) f[u] = __ldcs(x + lo + tid + u * 256);
+        const RowGrad q(p, r);
+        const int tok = q.t >= lo && q.t < hi ? (int)(q.t - lo) : -1;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = tid + u * 256;
+            if (j < n) __stcs(d + j, q.none ? 0.0f : q.at<ENT>(f[u]) - (j == tok ? q.g : 0.0f));
+        }
     }
 }
 
 // A warp a row.
+template <bool ENT>
 __global__ void __launch_bounds__(256) lp_bwd_warp_kernel(LpBwd p) {
     const int lane = threadIdx.x & 31;
     for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < p.rows; r += (int64_t)gridDim.x * 8) {
         const float* x = p.x + p.xm.offset(r);
         float* dx = p.dx + r * p.V;
         const RowGrad q(p, r);
-        for (int j = lane; j < p.V; j += 32) dx[j] = q.at(x[j], j);
+        for (int j = lane; j < p.V; j += 32) {
+            float y = q.none ? 0.0f : q.at<ENT>(x[j]);
+            if (j == q.t && !q.none) y -= q.g;
+            dx[j] = y;
+        }
     }
 }
 
@@ -530,12 +700,23 @@ int launch_warp(const LpFwd& p, cudaStream_t s) {
     return check_launch(kFwd);
 }
 
-template <int T>
-int launch_row(const LpFwd& p, int C, cudaStream_t s) {
-    if (p.rows * C > INT32_MAX) return set_error(TLC_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+// 256 threads and a ring of 48 KB a block: three blocks an SM.
+constexpr int ROW_T = 256;
+constexpr int ROW_BLOCKS = 3;
+
+int launch_row(const LpFwd& p, cudaStream_t s) {
+    constexpr size_t smem = sizeof(float4) * STAGES * BATCH * ROW_T;
+    static DeviceOnce once;
+    TLC_TRY(smem_limit_once(once, lp_row_kernel<ROW_T>, (int)smem));
+    const int64_t slots = (int64_t)sm_count() * ROW_BLOCKS;
+    // a cluster a row while the rows alone leave more than half the slots empty,
+    // down to 4096 logits a block
+    int C = 1;
+    while (C < 8 && p.rows * C * 2 <= slots && p.V / (2 * C) >= 4096) C *= 2;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(p.rows * C));
-    cfg.blockDim = dim3(T);
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, slots / C)) * C));
+    cfg.blockDim = dim3(ROW_T);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -543,7 +724,7 @@ int launch_row(const LpFwd& p, int C, cudaStream_t s) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = C > 1 ? 1 : 0;
-    TLC_CUDA_TRY(cudaLaunchKernelEx(&cfg, lp_row_kernel<T>, p, C));
+    TLC_CUDA_TRY(cudaLaunchKernelEx(&cfg, lp_row_kernel<ROW_T>, p, C));
     count_launch();
     return check_launch(kFwd);
 }
@@ -633,9 +814,7 @@ extern "C" int tlc_token_logprobs(const tlc_tensor* logits, const tlc_index* tok
     if (p.V <= 128) return launch_warp<4>(p, s);
     if (p.V <= 512) return launch_warp<16>(p, s);
     if (p.V <= 1024) return launch_warp<32>(p, s);
-    int C = 1;
-    while (C < 8 && p.rows * C * 2 <= 148 && p.V / (2 * C) >= 2048) C *= 2;
-    return C > 1 ? launch_row<512>(p, C, s) : launch_row<256>(p, C, s);
+    return launch_row(p, s);
 }
 
 extern "C" int tlc_token_logprobs_backward(const tlc_tensor* logits, const tlc_index* tokens,
@@ -692,7 +871,11 @@ extern "C" int tlc_token_logprobs_backward(const tlc_tensor* logits, const tlc_i
     p.V = (int)vx.cols;
     p.scale = scale;
     if (p.V <= 1024) {
-        lp_bwd_warp_kernel<<<(unsigned)std::min<int64_t>((p.rows + 7) / 8, INT32_MAX), 256, 0, s>>>(p);
+        const unsigned grid = (unsigned)std::min<int64_t>((p.rows + 7) / 8, INT32_MAX);
+        if (p.h)
+            lp_bwd_warp_kernel<true><<<grid, 256, 0, s>>>(p);
+        else
+            lp_bwd_warp_kernel<false><<<grid, 256, 0, s>>>(p);
     } else {
         const int pieces = (p.V + BW - 1) / BW;
         if (p.rows * pieces > INT32_MAX)
@@ -702,10 +885,14 @@ extern "C" int tlc_token_logprobs_backward(const tlc_tensor* logits, const tlc_i
                          (p.rows == 1 || (p.xm.nd == 1 && (p.xm.st[0] - p.V) % 4 == 0) ||
                           (p.V % 4 == 0 && p.xm.multiple_of(4)));
         const unsigned grid = (unsigned)(p.rows * pieces);
-        if (vec)
-            lp_bwd_kernel<true><<<grid, 256, 0, s>>>(p, pieces);
+        if (vec && p.h)
+            lp_bwd_kernel<true, true><<<grid, 256, 0, s>>>(p, pieces);
+        else if (vec)
+            lp_bwd_kernel<true, false><<<grid, 256, 0, s>>>(p, pieces);
+        else if (p.h)
+            lp_bwd_kernel<false, true><<<grid, 256, 0, s>>>(p, pieces);
         else
-            lp_bwd_kernel<false><<<grid, 256, 0, s>>>(p, pieces);
+            lp_bwd_kernel<false, false><<<grid, 256, 0, s>>>(p, pieces);
     }
     count_launch();
     return check_launch(kBwd);

@@ -198,6 +198,14 @@ inline int no_overlap(const char* op, const char* out_name, const Extent& out, c
     return set_error(TLC_ERR_INVALID_ARGUMENT, std::string(op) + ": " + out_name + " overlaps " + in_name);
 }
 
+inline int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+        return 148;
+    return sms;
+}
+
 // ---- device helpers --------------------------------------------------------------------
 
 template <int VEC>
@@ -211,7 +219,7 @@ struct FloatVec<4> {
     using T = float4;
 };
 
-// VEC floats at p (16-byte aligned where VEC is 4).  __ldcs: read once.
+// VEC floats at p (16-byte aligned where VEC is 4).  load_once, store_once: streaming.
 template <int VEC>
 __device__ __forceinline__ void load_vec(const float* p, float (&v)[VEC]) {
     if constexpr (VEC == 4) {
@@ -236,6 +244,14 @@ __device__ __forceinline__ void store_vec(float* p, const float (&v)[VEC]) {
         *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     else
         *p = v[0];
+}
+
+template <int VEC>
+__device__ __forceinline__ void store_once(float* p, const float (&v)[VEC]) {
+    if constexpr (VEC == 4)
+        __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+    else
+        __stcs(p, v[0]);
 }
 
 // Sums of N values over a warp, in every lane.

@@ -597,7 +597,9 @@ def token_logprobs(logits, tokens=None, scale=1.0, top=0, need_entropy=True, nee
     vx, vt = _fview(logits, dev, "logits"), _iview(tokens, dev, "tokens")
     lead = logits.shape[:-1]
     logp = logits.new_empty(lead) if tokens is not None else None
-    entropy = logits.new_empty(lead) if need_entropy else None
+    entropy = None
+    if need_entropy:  # empty_like is the cheaper call
+        entropy = logits.new_empty(lead) if logp is None else _torch.empty_like(logp)
     stats = logits.new_empty((*lead, 2)) if need_stats else None
     top_logp = top_tokens = None
     if top:
