@@ -32,10 +32,10 @@ struct EmbFwd {
     float scale;
 };
 
-// A warp copies EV vectors a lane of one row.  Rows and results are read and
-// written once: streaming loads and stores leave the L2 to the other tensors.
-constexpr int EV = 4;
-template <int VEC>
+// A warp copies EV vectors a lane of one row: 2 KB, whatever the vector.  Rows
+// and results are read and written once: streaming loads and stores leave the
+// L2 to the other tensors.
+template <int VEC, int EV = 16 / VEC>
 __global__ void __launch_bounds__(256) embed_kernel(EmbFwd p, int pieces) {
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * 8;
@@ -517,7 +517,7 @@ int check_scale(float scale, const char* op) {
 
 template <int VEC>
 int launch_embed(const EmbFwd& p, cudaStream_t s) {
-    const int pieces = (p.D + 32 * EV * VEC - 1) / (32 * EV * VEC);
+    const int pieces = (p.D + 511) / 512;
     const int64_t want = (p.n * pieces + 7) / 8;
     embed_kernel<VEC><<<(unsigned)std::min<int64_t>(want, INT32_MAX), 256, 0, s>>>(p, pieces);
     count_launch();

@@ -109,8 +109,10 @@ struct Run {
 // Adds values to a run, two at a time: 9 instructions for two values.
 struct PairRun {
     float m = -INFINITY;
-    float rest = -INFINITY;  // the maximum of the batches other than number `where`, which has m
-    int where = 0;
+    // batch `where` has m, batch `where2` the second largest of the batches' maxima, `rest` is the
+    // largest of the others' (all three NaN from the first NaN on)
+    float second = -INFINITY, rest = -INFINITY;
+    int where = 0, where2 = 0;
     Pair l, w, a2;
     float a;
     __device__ __forceinline__ explicit PairRun(float scale2) : l(0), w(0), a2(pair(scale2, scale2)), a(scale2) {}
@@ -126,9 +128,12 @@ struct PairRun {
                 w = mul2(pair(c, c), fma2(pair(y, y), l, w));
                 l = mul2(pair(c, c), l);
             }
-            rest = max_nan(rest, m);
-            m = to;
-            where = batch;
+            rest = max_nan(rest, second);
+            second = m, where2 = where;
+            m = to, where = batch;
+        } else if (top > second) {
+            rest = max_nan(rest, second);
+            second = top, where2 = batch;
         } else {
             rest = max_nan(rest, top);
         }
@@ -204,6 +209,7 @@ struct LpFwd {
 struct Asked {
     int64_t t = -1;
     float x = 0.0f;
+    Asked() = default;
     __device__ __forceinline__ Asked(const LpFwd& p, int64_t r, const float* row) {
         if (!p.logp) return;
         t = p.tok.get(r);
@@ -241,67 +247,12 @@ __device__ __forceinline__ void top_result(const LpFwd& p, int64_t r, int i, uin
         static_cast<int32_t*>(p.top_tok)[r * p.top + i] = (int32_t)j;
 }
 
-// ---- a row for a warp -------------------------------------------------------------------
+// ---- the copies ahead -------------------------------------------------------------------
 
-// V <= 32 * VPT, the values in registers (element 32 i + lane).
-template <int VPT>
-__global__ void __launch_bounds__(256) lp_warp_kernel(LpFwd p) {
-    const int lane = threadIdx.x & 31;
-    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < p.rows; r += (int64_t)gridDim.x * 8) {
-        const float* x = p.x + p.xm.offset(r);
-        float v[VPT];
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) v[i] = 32 * i + lane < p.V ? __ldcs(x + 32 * i + lane) : -INFINITY;
-        PairRun own(p.a);
-        own.add(v, 0);  // a lane without values of its own counts -inf: nothing
-        const Run s = warp_run(own.sum(), p.a);
-        if (lane == 0) row_results(p, r, Asked(p, r, x), s);
-        if (p.top) {
-            const float log_l = s.m == -INFINITY ? 0.0f : logf(s.l);
-            uint64_t last = ~0ull;  // the key picked before
-            for (int i = 0; i < p.top; ++i) {
-                uint64_t best = 0;
-#pragma unroll
-                for (int q = 0; q < VPT; ++q) {
-                    const uint32_t j = 32 * q + lane;
-                    if (j < (uint32_t)p.V) {
-                        const uint64_t k = key_of(v[q], j);
-                        if (k < last && k > best) best = k;
-                    }
-                }
-                const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
-                const uint32_t lo =
-                    __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
-                last = ((uint64_t)hi << 32) | lo;
-                if (lane == 0) top_result(p, r, i, last, s.m, log_l);
-            }
-        }
-    }
-}
-
-// ---- a row for a block or a cluster of blocks ----------------------------------------------
-
-constexpr int CAP = 512;  // candidates for the alternatives that a block keeps
-constexpr int BATCH = 4;  // float4 that a thread takes at once
+constexpr int BATCH = 4;   // float4 that a thread takes at once
 constexpr int STAGES = 3;  // batches in shared memory or on their way to it
 
-template <int T>
-struct LpSmem {
-    float m[T / 32], l[T / 32], w[T / 32];
-    float row_m, row_l, row_w;         // the block's sums, read by the cluster's first block
-    uint32_t group[64];
-    uint32_t bound;
-    int threads, found;
-    uint16_t look[T];                  // threads whose values reach the bound
-    int16_t batch[T];                  // and in which batch: a number, -1 (the single value), -2 (any)
-    uint64_t cand[CAP];
-    uint64_t best[kMaxTop];            // the block's alternatives, in order
-    uint64_t all[8 * kMaxTop];         // the cluster's, in its first block
-    uint32_t hist[256];
-    int bin, need;
-};
-
-// A block's part of a row: the first `head` values singly up to a 16-byte
+// A block's (or warp's) part of a row: the first `head` values singly up to a 16-byte
 // boundary, then `vecs` float4, then `tail` values.
 struct Part {
     const float* x;  // the part's first value
@@ -326,9 +277,227 @@ struct Part {
     }
 };
 
+// The values of a thread's rows, batch by batch, through a ring of asynchronous
+// copies that runs across the rows' ends, so that the memory stays busy while a
+// row's results are put together.  T threads share a row; a thread copies what
+// it reads itself, which needs no barrier.
+template <int T>
+struct Feed {
+    float4* ring;  // [STAGES][BATCH], this thread's float4 `pitch` apart
+    int pitch, t;
+    const LpFwd& p;
+    int lo, hi;
+    int64_t row, step;
+    int at = 0, stage = 0;
+    Part part;
+    __device__ __forceinline__ Feed(float4* ring_, int pitch_, int t_, const LpFwd& p_, int lo_, int hi_, int64_t first,
+                                    int64_t step_)
+        : ring(ring_), pitch(pitch_), t(t_), p(p_), lo(lo_), hi(hi_), row(first), step(step_),
+          part(p_.x + (first < p_.rows ? p_.xm.offset(first) : 0), lo_, hi_) {
+#pragma unroll
+        for (int q = 0; q < STAGES; ++q) fetch(q);
+    }
+    __device__ __forceinline__ void fetch(int to) {
+        if (row < p.rows) {
+            const float4* from = reinterpret_cast<const float4*>(part.x + part.head);
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                const int i = at + t + u * T;
+                if (i < part.vecs)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
+                                     __cvta_generic_to_shared(ring + (to * BATCH + u) * pitch))),
+                                 "l"(from + i)
+                                 : "memory");
+            }
+            at += BATCH * T;
+            if (at >= part.vecs) {  // every row has one batch at least
+                at = 0;
+                row += step;
+                if (row < p.rows) part = Part(p.x + p.xm.offset(row), lo, hi);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // all of one row's batches, then its single value
+    __device__ __forceinline__ void add_row(const Part& now, PairRun& own) {
+        const int alone_at = now.single(t);
+        const float alone = alone_at >= 0 ? now.x[alone_at] : -INFINITY;
+        int batch = 0;
+        do {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+            float v[4 * BATCH];
+#pragma unroll
+            for (int u = 0; u < BATCH; ++u) {
+                float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if ((batch * BATCH + u) * T + t < now.vecs) f = ring[(stage * BATCH + u) * pitch];
+                v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
+            }
+            fetch(stage);  // into what was just read
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            own.add(v, batch);
+            ++batch;
+        } while (batch * BATCH * T < now.vecs);
+        if (alone_at >= 0) {
+            const float v[1] = {alone};
+            own.add(v, -1);
+        }
+    }
+    __device__ __forceinline__ void end() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+};
+
+// One batch of thread t's values, seen again by that thread (-1: its single value).
+template <int T, class F>
+__device__ __forceinline__ void look_at_batch(const Part& part, int t, int batch, F&& take) {
+    if (batch < 0) {
+        const int at = part.single(t);
+        take(part.x[at], at);
+        return;
+    }
+    float4 f[BATCH];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+        const int i = (batch * BATCH + u) * T + t;
+        if (i < part.vecs) f[u] = part.vec(i);
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+        const int i = (batch * BATCH + u) * T + t, at = part.head + 4 * i;
+        if (i < part.vecs) {
+            take(f[u].x, at);
+            take(f[u].y, at + 1);
+            take(f[u].z, at + 2);
+            take(f[u].w, at + 3);
+        }
+    }
+}
+// The float4 [begin, end) of thread t's values, and its single one if asked,
+// seen again by a warp together.
+template <int T, class F>
+__device__ __forceinline__ void look_together(const Part& part, int t, int begin, int end, bool alone, int lane, F&& take) {
+    for (int i = begin + t + T * lane; i < end; i += T * 32) {
+        const float4 f = part.vec(i);
+        const int at = part.head + 4 * i;
+        take(f.x, at);
+        take(f.y, at + 1);
+        take(f.z, at + 2);
+        take(f.w, at + 3);
+    }
+    if (alone && lane == 0) {
+        const int at = part.single(t);
+        if (at >= 0) take(part.x[at], at);
+    }
+}
+
+// ---- a row for a warp -------------------------------------------------------------------
+
+constexpr int WARP_CAP = 128;  // candidates for the alternatives that a warp keeps
+constexpr int BOUND_BITS = 16;  // of a bound's 32: sign, exponent, 7 of the mantissa
+
+// A warp a row, 8 rows a block at once.
+template <bool TOP>
+__global__ void __launch_bounds__(256, 3) lp_warp_kernel(LpFwd p) {
+    extern __shared__ __align__(16) float4 ring[];  // [STAGES][BATCH][256]
+    __shared__ uint64_t cands[TOP ? 8 : 1][TOP ? WARP_CAP : 1];
+    __shared__ int founds[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t first = blockIdx.x + (int64_t)gridDim.x * warp, step = (int64_t)gridDim.x * 8;
+    Feed<32> feed(ring + threadIdx.x, 256, lane, p, 0, p.V, first, step);
+    for (int64_t r = first; r < p.rows; r += step) {
+        const float* x = p.x + p.xm.offset(r);
+        const Part part(x, 0, p.V);
+        const Asked asked = lane == 0 ? Asked(p, r, x) : Asked();
+        PairRun own(p.a);
+        feed.add_row(part, own);
+        const Run s = warp_run(own.sum(), p.a);
+        if (lane == 0) row_results(p, r, asked, s);
+        if constexpr (TOP) {
+            uint64_t* cand = cands[warp];
+            const float log_l = s.m == -INFINITY ? 0.0f : logf(s.l);
+            int found = WARP_CAP + 1;
+            if (s.m == s.m) {
+                // Each lane has three maxima of disjoint sets of its values.  What `top` of
+                // these 96 reach, `top` values reach: the highest such bound, bit by bit.
+                const uint32_t most = order_of(own.m), second = order_of(own.second), rest = order_of(own.rest);
+                uint32_t bound = 0;
+#pragma unroll
+                for (int bit = 31; bit >= 32 - BOUND_BITS; --bit) {
+                    const uint32_t to = bound | (1u << bit);
+                    const int reach = __popc(__ballot_sync(0xffffffffu, most >= to)) +
+                                      __popc(__ballot_sync(0xffffffffu, second >= to)) +
+                                      __popc(__ballot_sync(0xffffffffu, rest >= to));
+                    if (reach >= p.top) bound = to;
+                }
+                if (lane == 0) founds[warp] = 0;
+                __syncwarp();
+                auto take = [&](float v, int at) {
+                    if (order_of(v) >= bound) {
+                        const int c = atomicAdd(&founds[warp], 1);
+                        if (c < WARP_CAP) cand[c] = key_of(v, (uint32_t)at);
+                    }
+                };
+                // a lane looks at its one or two batches itself, at more with the others' help
+                const bool many = rest >= bound;
+                if (most >= bound && !many) look_at_batch<32>(part, lane, own.where, take);
+                if (second >= bound && !many) look_at_batch<32>(part, lane, own.where2, take);
+                __syncwarp();
+                for (uint32_t left = __ballot_sync(0xffffffffu, many); left; left &= left - 1)
+                    look_together<32>(part, __ffs(left) - 1, 0, part.vecs, true, lane, take);
+                __syncwarp();
+                found = founds[warp];
+            }
+            if (found <= WARP_CAP) {
+                for (int c = lane; c < found; c += 32) {
+                    const uint64_t key = cand[c];
+                    int before = 0;
+#pragma unroll 4
+                    for (int o = 0; o < found; ++o) before += cand[o] > key;
+                    if (before < p.top) top_result(p, r, before, key, s.m, log_l);
+                }
+            } else {
+                // NaN, or too many equal values: one alternative a round, the largest key below the last
+                uint64_t last = ~0ull;
+                for (int i = 0; i < p.top; ++i) {
+                    uint64_t best = 0;
+                    for (int j = lane; j < p.V; j += 32) {
+                        const uint64_t k = key_of(x[j], (uint32_t)j);
+                        if (k < last && k > best) best = k;
+                    }
+                    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32));
+                    const uint32_t lo =
+                        __reduce_max_sync(0xffffffffu, (uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+                    last = ((uint64_t)hi << 32) | lo;
+                    if (lane == 0) top_result(p, r, i, last, s.m, log_l);
+                }
+            }
+            __syncwarp();  // the list is written again
+        }
+    }
+    feed.end();
+}
+
+// ---- a row for a block or a cluster of blocks ----------------------------------------------
+
+constexpr int CAP = 512;  // candidates for the alternatives that a block keeps
+
+template <int T>
+struct LpSmem {
+    float m[T / 32], l[T / 32], w[T / 32];
+    float row_m, row_l, row_w;         // the block's sums, read by the cluster's first block
+    uint32_t group[64];
+    uint32_t bound;
+    int threads, found;
+    uint16_t look[T];                  // threads whose values reach the bound
+    int batch[T];                      // and in which batch: a number, -1 (the single value), -2 (any)
+    uint64_t cand[CAP];
+    uint64_t best[kMaxTop];            // the block's alternatives, in order
+    uint64_t all[8 * kMaxTop];         // the cluster's, in its first block
+    uint32_t hist[256];
+    int bin, need;
+};
+
 // The part's `k` largest keys in order, into sm.best (k <= part.n values; the
 // rest of sm.best is 0).  top: the largest value of this thread (-inf: none),
-// which its batch `where` has (-1: its single value), rest: of its others.
+// which its batch `where` has (-1: its single value), rest: that of the others.
 template <int T>
 __device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top, float rest, int where) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -351,36 +520,24 @@ __device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top, floa
     }
     __syncthreads();
     const uint32_t bound = sm.bound;
-    // mostly no other batch of the thread reaches the bound: then one is looked at, else all
-    if (order_of(top) >= bound) {
-        const int c = atomicAdd(&sm.threads, 1);
-        sm.look[c] = (uint16_t)tid;
-        sm.batch[c] = (int16_t)(order_of(rest) >= bound ? -2 : where);
-    }
-    __syncthreads();
-    const int threads = sm.threads;
     auto take = [&](float v, int at) {
         if (order_of(v) >= bound) {
             const int c = atomicAdd(&sm.found, 1);
             if (c < CAP) sm.cand[c] = key_of(v, (uint32_t)(part.first + at));
         }
     };
+    // mostly no other batch of the thread reaches the bound: then one is looked at, else all
+    if (order_of(top) >= bound) {
+        const int c = atomicAdd(&sm.threads, 1);
+        sm.look[c] = (uint16_t)tid;
+        sm.batch[c] = order_of(rest) >= bound ? -2 : where;
+    }
+    __syncthreads();
+    const int threads = sm.threads;
     for (int q = warp; q < threads; q += T / 32) {
-        const int t = sm.look[q], only = sm.batch[q];
-        const int begin = only == -2 ? 0 : only == -1 ? part.vecs : only * BATCH * T;
-        const int end = only == -2 ? part.vecs : only == -1 ? 0 : min(part.vecs, begin + BATCH * T);
-        for (int i = begin + t + T * lane; i < end; i += T * 32) {
-            const float4 f = part.vec(i);
-            const int at = part.head + 4 * i;
-            take(f.x, at);
-            take(f.y, at + 1);
-            take(f.z, at + 2);
-            take(f.w, at + 3);
-        }
-        if (lane == 0 && only < 0) {
-            const int at = part.single(t);
-            if (at >= 0) take(part.x[at], at);
-        }
+        const int batch = sm.batch[q], begin = batch >= 0 ? batch * BATCH * T : 0;
+        const int end = batch >= 0 ? min(part.vecs, begin + BATCH * T) : batch == -1 ? 0 : part.vecs;
+        look_together<T>(part, sm.look[q], begin, end, batch < 0, lane, take);
     }
     __syncthreads();
     int found = sm.found;
@@ -437,10 +594,7 @@ __device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top, floa
 }
 
 // C blocks a row (1, or the cluster's size), T threads a block, each block (or
-// cluster) with several rows.  The rows' values come through a ring of
-// asynchronous copies that runs across the rows' ends, so that the memory stays
-// busy while a row's results are put together; a thread copies what it reads
-// itself, which needs no barrier.
+// cluster) with several rows.
 template <int T>
 __global__ void __launch_bounds__(T) lp_row_kernel(LpFwd p, int C) {
     extern __shared__ __align__(16) float4 ring[];  // [STAGES][BATCH][T]
@@ -451,61 +605,13 @@ __global__ void __launch_bounds__(T) lp_row_kernel(LpFwd p, int C) {
     const int per = ((p.V + C - 1) / C + 31) & ~31;
     const int lo = (int)min((int64_t)p.V, (int64_t)rank * per), hi = (int)min((int64_t)p.V, (int64_t)lo + per);
 
-    int64_t ahead_row = first;  // the next batch to copy
-    int ahead_at = 0;
-    Part ahead(p.x + p.xm.offset(first), lo, hi);
-    auto fetch = [&](int stage) {
-        if (ahead_row < p.rows) {
-            const float4* from = reinterpret_cast<const float4*>(ahead.x + ahead.head);
-#pragma unroll
-            for (int u = 0; u < BATCH; ++u) {
-                const int i = ahead_at + tid + u * T;
-                if (i < ahead.vecs)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
-                                     __cvta_generic_to_shared(&ring[(stage * BATCH + u) * T + tid]))),
-                                 "l"(from + i)
-                                 : "memory");
-            }
-            ahead_at += BATCH * T;
-            if (ahead_at >= ahead.vecs) {
-                ahead_at = 0;
-                ahead_row += step;
-                if (ahead_row < p.rows) ahead = Part(p.x + p.xm.offset(ahead_row), lo, hi);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int q = 0; q < STAGES; ++q) fetch(q);
-    int stage = 0;
+    Feed<T> feed(ring + tid, T, tid, p, lo, hi, first, step);
     for (int64_t r = first; r < p.rows; r += step) {
         const float* x = p.x + p.xm.offset(r);
         const Part part(x, lo, hi);
-        const int at = part.single(tid);
-        const float alone = at >= 0 ? part.x[at] : -INFINITY;
-        const bool asks = tid == 0 && rank == 0;
-        const Asked asked = asks ? Asked(p, r, x) : Asked(LpFwd{}, 0, nullptr);
+        const Asked asked = tid == 0 && rank == 0 ? Asked(p, r, x) : Asked();
         PairRun own(p.a);
-        int batch = 0;
-        do {  // one batch even of a row without float4, as fetch() has it
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-            float v[4 * BATCH];
-#pragma unroll
-            for (int u = 0; u < BATCH; ++u) {
-                const int i = (batch * BATCH + u) * T + tid;
-                float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if (i < part.vecs) f = ring[(stage * BATCH + u) * T + tid];
-                v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
-            }
-            fetch(stage);  // into what was just read
-            stage = stage + 1 == STAGES ? 0 : stage + 1;
-            own.add(v, batch);
-            ++batch;
-        } while (batch * BATCH * T < part.vecs);
-        if (at >= 0) {
-            const float v[1] = {alone};
-            own.add(v, -1);
-        }
+        feed.add_row(part, own);
         const Run s = warp_run(own.sum(), p.a);
         if (lane == 0) sm.m[warp] = s.m, sm.l[warp] = s.l, sm.w[warp] = s.w;
         __syncthreads();
@@ -517,7 +623,7 @@ __global__ void __launch_bounds__(T) lp_row_kernel(LpFwd p, int C) {
         }
         const int k = min(p.top, part.n);
         if (k > 0)
-            part_top(sm, part, k, own.m, own.rest, own.where);
+            part_top(sm, part, k, own.m, max_nan(own.second, own.rest), own.where);
         else if (p.top > 0 && tid < kMaxTop)
             sm.best[tid] = 0;
         __syncthreads();
@@ -570,7 +676,7 @@ __global__ void __launch_bounds__(T) lp_row_kernel(LpFwd p, int C) {
         }
         cluster_sync();  // the first block has read the others' shared memory
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    feed.end();
 }
 
 // ---- the gradient ---------------------------------------------------------------------------
@@ -617,27 +723,29 @@ struct RowGrad {
     }
 };
 
-// 256 threads for a run of BW values of one row, all loaded before the first is
-// written.
-constexpr int BW = 16384;
-template <bool VEC, bool ENT>
+// T threads take a run of at most 64 T values of one row, all of them asked for
+// before the row's constants (which take as long to come) and before the first
+// result is written; nobody waits for anybody.
+constexpr int BWD_RUN = 64;
+template <bool VEC, bool ENT, int T>
 __global__ void __launch_bounds__(256) lp_bwd_kernel(LpBwd p, int pieces) {
-    const int64_t r = blockIdx.x / pieces;
-    const int lo = (int)(blockIdx.x - r * pieces) * BW, hi = min(p.V, lo + BW);
+    constexpr int BW = BWD_RUN * T;
+    const int t = threadIdx.x & (T - 1);
+    const int64_t unit = (int64_t)blockIdx.x * (256 / T) + threadIdx.x / T, r = unit / pieces;
+    if (r >= p.rows) return;
+    const int lo = (int)(unit - r * pieces) * BW, hi = min(p.V, lo + BW);
     const float* x = p.x + p.xm.offset(r);
     float* d = p.dx + r * p.V + lo;
-    const int n = hi - lo, tid = threadIdx.x;
-    // the values are asked for before the row's constants, which take as long
     if constexpr (VEC) {
         const Part part(x, lo, hi);
         const float4* from = reinterpret_cast<const float4*>(part.x + part.head);
         float4* to = reinterpret_cast<float4*>(d + part.head);
-        constexpr int U = BW / 4 / 256;
+        constexpr int U = BWD_RUN / 4;
         float4 f[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (tid + u * 256 < part.vecs) f[u] = __ldcs(from + tid + u * 256);
-        const int at = part.single(tid);
+            if (t + u * T < part.vecs) f[u] = __ldcs(from + t + u * T);
+        const int at = part.single(t);
         const float alone = at >= 0 ? part.x[at] : 0.0f;
         const RowGrad q(p, r);
         const int tok = q.t >= lo && q.t < hi ? (int)(q.t - lo) : -1;  // the token's place here
@@ -645,7 +753,7 @@ __global__ void __launch_bounds__(256) lp_bwd_kernel(LpBwd p, int pieces) {
         const int tv = tok < part.head ? -1 : (tok - part.head) >> 2;  // the token's vector
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = tid + u * 256;
+            const int i = t + u * T;
             if (i < part.vecs) {
                 float4 y;
                 y.x = q.at<ENT>(f[u].x), y.y = q.at<ENT>(f[u].y), y.z = q.at<ENT>(f[u].z), y.w = q.at<ENT>(f[u].w);
@@ -661,53 +769,61 @@ __global__ void __launch_bounds__(256) lp_bwd_kernel(LpBwd p, int pieces) {
             }
         }
     } else {
-        constexpr int U = BW / 256;
+        const int n = hi - lo;
+        constexpr int U = BWD_RUN;
         float f[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (tid + u * 256 < n) f[u] = __ldcs(x + lo + tid + u * 256);
+            if (t + u * T < n) f[u] = __ldcs(x + lo + t + u * T);
         const RowGrad q(p, r);
         const int tok = q.t >= lo && q.t < hi ? (int)(q.t - lo) : -1;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = tid + u * 256;
+            const int j = t + u * T;
             if (j < n) __stcs(d + j, q.none ? 0.0f : q.at<ENT>(f[u]) - (j == tok ? q.g : 0.0f));
         }
     }
 }
 
-// A warp a row.
-template <bool ENT>
-__global__ void __launch_bounds__(256) lp_bwd_warp_kernel(LpBwd p) {
-    const int lane = threadIdx.x & 31;
-    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < p.rows; r += (int64_t)gridDim.x * 8) {
-        const float* x = p.x + p.xm.offset(r);
-        float* dx = p.dx + r * p.V;
-        const RowGrad q(p, r);
-        for (int j = lane; j < p.V; j += 32) {
-            float y = q.none ? 0.0f : q.at<ENT>(x[j]);
-            if (j == q.t && !q.none) y -= q.g;
-            dx[j] = y;
-        }
-    }
-}
-
-template <int VPT>
-int launch_warp(const LpFwd& p, cudaStream_t s) {
-    const unsigned grid = (unsigned)std::min<int64_t>((p.rows + 7) / 8, INT32_MAX);
-    lp_warp_kernel<VPT><<<grid, 256, 0, s>>>(p);
+template <int T>
+int launch_bwd(const LpBwd& p, bool vec, cudaStream_t s) {
+    const int pieces = (p.V + BWD_RUN * T - 1) / (BWD_RUN * T);
+    const int64_t blocks = (p.rows * pieces + 256 / T - 1) / (256 / T);
+    if (blocks > INT32_MAX) return set_error(TLC_ERR_UNSUPPORTED, "token_logprobs_backward: too many rows");
+    const unsigned grid = (unsigned)blocks;
+    if (vec && p.h)
+        lp_bwd_kernel<true, true, T><<<grid, 256, 0, s>>>(p, pieces);
+    else if (vec)
+        lp_bwd_kernel<true, false, T><<<grid, 256, 0, s>>>(p, pieces);
+    else if (p.h)
+        lp_bwd_kernel<false, true, T><<<grid, 256, 0, s>>>(p, pieces);
+    else
+        lp_bwd_kernel<false, false, T><<<grid, 256, 0, s>>>(p, pieces);
     count_launch();
-    return check_launch(kFwd);
+    return check_launch(kBwd);
 }
 
 // 256 threads and a ring of 48 KB a block: three blocks an SM.
 constexpr int ROW_T = 256;
 constexpr int ROW_BLOCKS = 3;
+constexpr size_t kRing = sizeof(float4) * STAGES * BATCH * ROW_T;
+
+int launch_warp(const LpFwd& p, cudaStream_t s) {
+    static DeviceOnce once[2];
+    TLC_TRY(smem_limit_once(once[0], lp_warp_kernel<false>, (int)kRing));
+    TLC_TRY(smem_limit_once(once[1], lp_warp_kernel<true>, (int)kRing));
+    const int64_t grid = std::min<int64_t>(p.rows, (int64_t)sm_count() * ROW_BLOCKS);
+    if (p.top)
+        lp_warp_kernel<true><<<(unsigned)grid, 256, kRing, s>>>(p);
+    else
+        lp_warp_kernel<false><<<(unsigned)grid, 256, kRing, s>>>(p);
+    count_launch();
+    return check_launch(kFwd);
+}
 
 int launch_row(const LpFwd& p, cudaStream_t s) {
-    constexpr size_t smem = sizeof(float4) * STAGES * BATCH * ROW_T;
     static DeviceOnce once;
-    TLC_TRY(smem_limit_once(once, lp_row_kernel<ROW_T>, (int)smem));
+    TLC_TRY(smem_limit_once(once, lp_row_kernel<ROW_T>, (int)kRing));
     const int64_t slots = (int64_t)sm_count() * ROW_BLOCKS;
     // a cluster a row while the rows alone leave more than half the slots empty,
     // down to 4096 logits a block
@@ -716,7 +832,7 @@ int launch_row(const LpFwd& p, cudaStream_t s) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(std::min<int64_t>(p.rows, std::max<int64_t>(1, slots / C)) * C));
     cfg.blockDim = dim3(ROW_T);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = kRing;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -811,9 +927,7 @@ extern "C" int tlc_token_logprobs(const tlc_tensor* logits, const tlc_index* tok
         p.top_tok = top_tokens->data;
         p.top_wide = top_tokens->bits == 64;
     }
-    if (p.V <= 128) return launch_warp<4>(p, s);
-    if (p.V <= 512) return launch_warp<16>(p, s);
-    if (p.V <= 1024) return launch_warp<32>(p, s);
+    if (p.V <= 1024 || (p.V <= 16384 && p.rows >= (int64_t)sm_count() * 8)) return launch_warp(p, s);
     return launch_row(p, s);
 }
 
@@ -870,30 +984,11 @@ extern "C" int tlc_token_logprobs_backward(const tlc_tensor* logits, const tlc_i
     p.rows = vx.rows;
     p.V = (int)vx.cols;
     p.scale = scale;
-    if (p.V <= 1024) {
-        const unsigned grid = (unsigned)std::min<int64_t>((p.rows + 7) / 8, INT32_MAX);
-        if (p.h)
-            lp_bwd_warp_kernel<true><<<grid, 256, 0, s>>>(p);
-        else
-            lp_bwd_warp_kernel<false><<<grid, 256, 0, s>>>(p);
-    } else {
-        const int pieces = (p.V + BW - 1) / BW;
-        if (p.rows * pieces > INT32_MAX)
-            return set_error(TLC_ERR_UNSUPPORTED, "token_logprobs_backward: too many rows");
-        // float4 where each row of x and dx starts at the same place within 16 bytes
-        const bool vec = (reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.dx)) % 16 == 0 &&
-                         (p.rows == 1 || (p.xm.nd == 1 && (p.xm.st[0] - p.V) % 4 == 0) ||
-                          (p.V % 4 == 0 && p.xm.multiple_of(4)));
-        const unsigned grid = (unsigned)(p.rows * pieces);
-        if (vec && p.h)
-            lp_bwd_kernel<true, true><<<grid, 256, 0, s>>>(p, pieces);
-        else if (vec)
-            lp_bwd_kernel<true, false><<<grid, 256, 0, s>>>(p, pieces);
-        else if (p.h)
-            lp_bwd_kernel<false, true><<<grid, 256, 0, s>>>(p, pieces);
-        else
-            lp_bwd_kernel<false, false><<<grid, 256, 0, s>>>(p, pieces);
-    }
-    count_launch();
-    return check_launch(kBwd);
+    // float4 where each row of x and dx starts at the same place within 16 bytes
+    const bool vec = (reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.dx)) % 16 == 0 &&
+                     (p.rows == 1 || (p.xm.nd == 1 && (p.xm.st[0] - p.V) % 4 == 0) ||
+                      (p.V % 4 == 0 && p.xm.multiple_of(4)));
+    // a block a run of a long row (4096 x 50001: 265 us, 296 by warps), a warp a run of a
+    // short one (8192 x 999: 17 us, 46 by blocks)
+    return p.V > 8192 ? launch_bwd<256>(p, vec, s) : launch_bwd<32>(p, vec, s);
 }
