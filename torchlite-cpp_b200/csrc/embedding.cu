@@ -94,7 +94,7 @@ struct SortArgs {
     uint2* b;          // [n], odd passes
     int* crossing;     // set to 0 here: the count of runs that cross chunks
     float* dw;         // rows to fill with zeros (NULL: none)
-    int D, vec;        // vec: rows start on 16 bytes
+    int D;
     int group_shift;   // rows are dealt to the blocks in groups of 2^group_shift, at least 2 KB each
 };
 
@@ -135,28 +135,42 @@ __device__ void sort_positions(const SortArgs& p, SortSmem& sm) {
         const bool last = pass + 1 == p.passes;
         const int shift = pass * p.bits;
         auto digit = [&](uint2 k) { return (k.x >> shift) & (uint32_t)(bins - 1); };
-        auto load = [&](int i) -> uint2 {
+        // keys first, first + step, ... below i1 (all loads before the first use)
+        auto load = [&](int first, int step, uint2 (&to)[ITEMS]) {
             if (pass == 0) {
-                const int64_t t = p.tok.get(i);
-                return make_uint2((uint32_t)(t >= 0 && t < p.rows ? t : p.rows), (uint32_t)i);
+                int64_t t[ITEMS];
+                p.tok.get(first, step, i1, t);
+#pragma unroll
+                for (int k = 0; k < ITEMS; ++k)
+                    to[k] = make_uint2((uint32_t)(t[k] >= 0 && t[k] < p.rows ? t[k] : p.rows),
+                                       (uint32_t)(first + k * step));
+            } else if (one) {
+#pragma unroll
+                for (int k = 0; k < ITEMS; ++k)
+                    if (first + k * step < i1) to[k] = sm.keys[first + k * step - i0];
+            } else {
+#pragma unroll
+                for (int k = 0; k < ITEMS; ++k)
+                    if (first + k * step < i1) to[k] = __ldcg(src + first + k * step);
             }
-            return one ? sm.keys[i - i0] : __ldcg(src + i);
         };
         // a tile's keys, and each key's place among its warp's of the same digit
         auto rank_tile = [&](int t0) {
             for (int d = lane; d < bins; d += 32) sm.warp[warp][d] = 0;
             const int w0 = t0 + warp * 32 * items + lane;
-#pragma unroll
-            for (int k = 0; k < ITEMS; ++k)
-                if (k < items && w0 + k * 32 < i1) kv[k] = load(w0 + k * 32);
+            load(w0, 32, kv);  // with fewer items a warp also reads its neighbours' keys, and leaves them
             __syncwarp();
 #pragma unroll
             for (int k = 0; k < ITEMS; ++k) {
                 if (k >= items) break;
                 const bool in = w0 + k * 32 < i1;
-                // lanes past the end match nobody's digit
-                const uint32_t d = in ? digit(kv[k]) : (uint32_t)(BINS + lane);
-                const uint32_t peers = __match_any_sync(0xffffffffu, d);
+                const uint32_t d = in ? digit(kv[k]) : 0u;
+                // the lanes with the same digit, by a vote for each of its bits
+                uint32_t peers = __ballot_sync(0xffffffffu, in);
+                for (int b = 0; b < p.bits; ++b) {
+                    const uint32_t vote = __ballot_sync(0xffffffffu, (d >> b) & 1u);
+                    peers &= (d >> b) & 1u ? vote : ~vote;
+                }
                 const uint32_t old = in ? sm.warp[warp][d] : 0u;
                 __syncwarp();
                 if (in && lane == 31 - __clz(peers)) sm.warp[warp][d] = old + __popc(peers);
@@ -202,7 +216,12 @@ __device__ void sort_positions(const SortArgs& p, SortSmem& sm) {
         } else {
             for (int d = tid; d < bins; d += SORT_T) sm.hist[d] = 0;
             __syncthreads();
-            for (int i = i0 + tid; i < i1; i += SORT_T) atomicAdd(&sm.hist[digit(load(i))], 1u);
+            for (int i = i0 + tid; i < i1; i += TILE) {
+                load(i, SORT_T, kv);
+#pragma unroll
+                for (int k = 0; k < ITEMS; ++k)
+                    if (i + k * SORT_T < i1) atomicAdd(&sm.hist[digit(kv[k])], 1u);
+            }
         }
         cluster_sync();  // counts in place; with one tile all keys are in registers as well
         // base[d] = keys of lower digits in the cluster + keys of d in lower blocks
@@ -257,9 +276,8 @@ __device__ void fill_absent(const SortArgs& p, FillSmem& sm, uint32_t cluster, u
     const int gs = p.group_shift;
     const int64_t span = (int64_t)blocks * ZROWS;  // rows whose marks fit at once
     // the lanes that share a row
-    const int units = p.vec ? p.D / 4 : p.D;
     int g = 1;
-    while (g < 32 && g < units) g <<= 1;
+    while (g < 32 && g * 4 < p.D) g <<= 1;
     for (int64_t lo = 0; lo < p.rows; lo += span) {
         const uint32_t rows = (uint32_t)min(span, p.rows - lo);
         const uint32_t groups = (rows + (1u << gs) - 1) >> gs;
@@ -268,13 +286,10 @@ __device__ void fill_absent(const SortArgs& p, FillSmem& sm, uint32_t cluster, u
         cluster_sync();
         for (int64_t i0 = (int64_t)rank * SORT_T + tid; i0 < p.n; i0 += CL * SORT_T * 4) {
             int64_t t[4];
+            p.tok.get(i0, CL * SORT_T, p.n, t);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int64_t i = i0 + (int64_t)k * CL * SORT_T;
-                t[k] = i < p.n ? p.tok.get(i) - lo : -1;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
+                t[k] -= lo;
                 if (t[k] < 0 || t[k] >= (int64_t)rows) continue;
                 const uint32_t group = (uint32_t)t[k] >> gs, turn = group / blocks, owner = group - turn * blocks;
                 if (owner / CL != cluster) continue;
@@ -291,12 +306,13 @@ __device__ void fill_absent(const SortArgs& p, FillSmem& sm, uint32_t cluster, u
             const uint32_t v = ((((q >> gs) * blocks) + me) << gs) | (q & ((1u << gs) - 1u));
             if (v >= rows) continue;
             float* row = p.dw + (lo + v) * p.D;
-            if (p.vec) {
-                for (int j = lane & (g - 1); j < units; j += g)
-                    __stcs(reinterpret_cast<float4*>(row) + j, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
-            } else {
-                for (int j = lane & (g - 1); j < units; j += g) __stcs(row + j, 0.0f);
-            }
+            // single values up to a 16-byte boundary and behind the last one, float4 between
+            const int head = min(p.D, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) >> 2);
+            const int vecs = (p.D - head) >> 2;
+            for (int j = lane & (g - 1); j < vecs; j += g)
+                __stcs(reinterpret_cast<float4*>(row + head) + j, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+            for (int j = lane & (g - 1); j < head; j += g) __stcs(row + j, 0.0f);
+            for (int j = head + 4 * vecs + (lane & (g - 1)); j < p.D; j += g) __stcs(row + j, 0.0f);
         }
         cluster_sync();  // before the marks are cleared again
     }
@@ -437,8 +453,9 @@ __global__ void __launch_bounds__(256) embed_join_kernel(SumArgs p, int slices) 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int runs = *p.crossing;
     const int64_t units = (int64_t)runs * slices;
-    for (int64_t u0 = (int64_t)blockIdx.x * 8; u0 < units; u0 += (int64_t)gridDim.x * 8) {
-        const int64_t u = u0 + warp;
+    // the block's warps take units far apart: frequent tokens, neighbours in the list, have long runs
+    for (int64_t u0 = blockIdx.x; u0 < units; u0 += (int64_t)gridDim.x * 8) {
+        const int64_t u = u0 + (int64_t)gridDim.x * warp;
         int count = 0;  // chunks behind the first
         if (u < units) {
             // neighbouring warps take different runs: the slices of a long one go to different blocks
@@ -649,7 +666,6 @@ extern "C" int tlc_embedding_backward(const tlc_tensor* grad, const tlc_index* t
         TLC_TRY(max_clusters(&clusters));
         q.dw = dweight->data;
         q.D = D;
-        q.vec = D % 4 == 0 && aligned_to(q.dw, 16);
         while (q.group_shift < 5 && ((int64_t)D * 4 << q.group_shift) < 2048) ++q.group_shift;
     } else {
         int unused;

@@ -26,64 +26,73 @@ struct LnFwd {
     float eps;
 };
 
-// THREADS threads a row (32: a warp for each row, 4 rows a block), VPT vectors
-// of VEC floats a thread: D <= THREADS * VPT * VEC.
+// THREADS threads a row (a block, or up to 32 neighbouring lanes of 4 warps), VPT
+// vectors of VEC floats a thread: D <= THREADS * VPT * VEC.  64 registers a
+// thread, so that 1024 threads are on an SM.
 template <int VEC, int VPT, int THREADS>
-__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) ln_fwd_kernel(LnFwd p) {
-    constexpr int RPB = THREADS == 32 ? 4 : 1;
+__global__ void __launch_bounds__(THREADS <= 32 ? 128 : THREADS, THREADS <= 32 ? 1 : 1024 / THREADS)
+    ln_fwd_kernel(LnFwd p) {
+    constexpr int RPB = THREADS <= 32 ? 128 / THREADS : 1;
     __shared__ float red[2][32];
-    const int t = THREADS == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const int sub = THREADS == 32 ? (threadIdx.x >> 5) : 0;
-    for (int64_t r = (int64_t)blockIdx.x * RPB + sub; r < p.rows; r += (int64_t)gridDim.x * RPB) {
-        const float* xr = p.x + p.xm.offset(r);
+    const int t = threadIdx.x % THREADS, sub = threadIdx.x / THREADS;
+    const int n = p.D / VEC;
+    const int whole = n / THREADS + (t < n % THREADS ? 1 : 0);  // this thread's vectors of a row
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < p.rows; r0 += (int64_t)gridDim.x * RPB) {
+        const int64_t r = r0 + sub;
+        const bool live = RPB == 1 || r < p.rows;  // lanes without a row take part in the sums
+        const int mine = live ? whole : 0;
+        const float* xr = p.x + (live ? p.xm.offset(r) : 0) + t * VEC;
         float v[VPT][VEC];
-        float s[1] = {0.0f};
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int j = (t + i * THREADS) * VEC;
-            if (j < p.D) {
-                load_once<VEC>(xr + j, v[i]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) v[i][k] = 0.0f;
-            }
-        }
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
+            if (i < mine) load_once<VEC>(xr + i * THREADS * VEC, v[i]);
+        float s[1] = {0.0f};
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) s[0] += v[i][k];
+        for (int i = 0; i < VPT; ++i)
+            if (i < mine)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) s[0] += v[i][k];
         group_sum<THREADS>(s, red[0]);
         const float mean = __fdiv_rn(s[0], (float)p.D);  // exact for rows of one value
         float q[1] = {0.0f};
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const bool in = (t + i * THREADS) * VEC < p.D;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                v[i][k] -= mean;
-                if (in) q[0] = fmaf(v[i][k], v[i][k], q[0]);
-            }
-        }
-        group_sum<THREADS>(q, red[1]);
-        const float rstd = __frsqrt_rn(__fdiv_rn(q[0], (float)p.D) + p.eps);
-        float* yr = p.out + r * p.D;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int j = (t + i * THREADS) * VEC;
-            if (j < p.D) {
-                float wv[VEC], bv[VEC], y[VEC];
-                if (p.w) load_vec<VEC>(p.w + j, wv);
-                if (p.b) load_vec<VEC>(p.b + j, bv);
+        for (int i = 0; i < VPT; ++i)
+            if (i < mine)
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
-                    y[k] = v[i][k] * rstd;
-                    if (p.w) y[k] *= wv[k];
-                    if (p.b) y[k] += bv[k];
+                    v[i][k] -= mean;
+                    q[0] = fmaf(v[i][k], v[i][k], q[0]);
                 }
-                store_vec<VEC>(yr + j, y);
-            }
+        group_sum<THREADS>(q, red[1]);
+        const float rstd = __frsqrt_rn(__fdiv_rn(q[0], (float)p.D) + p.eps);
+        float* yr = p.out + r * p.D + t * VEC;
+        const float* w = p.w + t * VEC;
+        const float* b = p.b + t * VEC;
+        if (p.w && p.b) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (i < mine) {
+                    float wv[VEC], bv[VEC];
+                    load_vec<VEC>(w + i * THREADS * VEC, wv);
+                    load_vec<VEC>(b + i * THREADS * VEC, bv);
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) v[i][k] = fmaf(v[i][k] * rstd, wv[k], bv[k]);
+                    store_once<VEC>(yr + i * THREADS * VEC, v[i]);
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (i < mine) {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) {
+                        v[i][k] *= rstd;
+                        if (p.w) v[i][k] *= w[i * THREADS * VEC + k];
+                        if (p.b) v[i][k] += b[i * THREADS * VEC + k];
+                    }
+                    store_once<VEC>(yr + i * THREADS * VEC, v[i]);
+                }
         }
-        if (p.stats && t == 0) {
+        if (p.stats && t == 0 && live) {
             p.stats[2 * r] = mean;
             p.stats[2 * r + 1] = rstd;
         }
@@ -130,21 +139,15 @@ struct LnBwd {
     int accumulate;
 };
 
-// One block an SM, 8 warps; W warps a row, 8 / W rows at a time.  Each lane
-// keeps the same columns for every row, so the sums for dw and db stay in its
-// registers until the end.  The rows come through a ring of STAGES rows of x
-// and g in shared memory, filled by asynchronous copies: a thread copies just
-// what it reads itself, so the ring needs no barrier, and rows far enough
-// ahead are always in flight although the registers allow only 8 warps.
-constexpr int BT = 256;
-
-template <int VEC>
-__device__ __forceinline__ void copy_async(float* dst, const float* src) {
-    const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
-    if constexpr (VEC == 4)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
+__device__ __forceinline__ void copy16(float* dst, const float* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void copy4(float* dst, const float* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src)
+                 : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -152,54 +155,106 @@ __device__ __forceinline__ void copies_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Rows of x and g kept in shared memory: what 192 KB hold, at most 8.
-template <int VEC, int VPT>
-constexpr int ring_stages() {
-    const int n = 192 * 1024 / (BT * VPT * VEC * 4 * 2);
-    return n < 8 ? n : 8;
-}
+// One block an SM, 16 warps; THREADS threads a row (8 lanes to the whole block),
+// 512 / THREADS rows at a time.  Each thread keeps the same columns for every
+// row, so the sums for dw and db stay in its registers until the end; up to 16
+// columns a thread, two an instruction (with 8 warps of 32 columns the loop's
+// code was fetched more slowly than it ran: half of all stalls), and 24 or 32,
+// with spills, only for rows that a block could not hold otherwise.
+//
+// The rows come through a ring of rows of x and g in shared memory, filled by
+// asynchronous copies, so that rows far enough ahead are always in flight
+// although the registers allow only 16 warps.  Where all rows start on 16 bytes
+// (VEC 4) a thread copies just what it reads itself, which needs no barrier.
+// Otherwise (VEC 1) the row's threads copy its aligned 16-byte pieces together,
+// single values at its ends, and meet before they read and before they refill.
+constexpr int BT = 512;
 
-template <int VEC, int VPT, int W>
+template <int VEC, int VPT, int THREADS>
+struct LnRing {
+    static constexpr int ROW = THREADS * VPT * VEC + (VEC == 1 ? 8 : 0);  // floats a row
+    static constexpr int SLOT = 2 * (BT / THREADS) * ROW;                 // x and g of the rows at a time
+    static constexpr int FIT = 200 * 1024 / (SLOT * 4);
+    static constexpr int STAGES = FIT < 8 ? FIT : 8;
+    static constexpr int BYTES = STAGES * SLOT * 4;
+};
+
+// The VPT * VEC values of a thread as pairs: value q is (vector q / VEC, element q % VEC).
+template <int VEC, int VPT, int THREADS>
 __global__ void __launch_bounds__(BT, 1) ln_bwd_kernel(LnBwd p) {
-    constexpr int S = ring_stages<VEC, VPT>();
-    constexpr int GROUPS = BT / 32 / W, THREADS = 32 * W;
-    extern __shared__ __align__(16) float ring[];  // [S][2][VPT][BT][VEC], then [GROUPS][2][D]
+    using R = LnRing<VEC, VPT, THREADS>;
+    constexpr int S = R::STAGES, GROUPS = BT / THREADS, W = THREADS > 32 ? THREADS / 32 : 1, N = VEC * VPT;
+    extern __shared__ __align__(16) float ring[];  // [S][GROUPS][2][ROW], then [GROUPS][2][D]
     __shared__ float red[2][GROUPS][2 * W];
     const int group = threadIdx.x / THREADS, t = threadIdx.x % THREADS, lane = threadIdx.x & 31;
     const float inv = 1.0f / (float)p.D;
-    float aw[VPT][VEC], ab[VPT][VEC], w[VPT][VEC];
+    const int vecs = p.D / VEC;
+    const int whole = vecs / THREADS + (t < vecs % THREADS ? 1 : 0);  // this thread's vectors of a row
+    Pair aw[N / 2], ab[N / 2], w[N / 2];
+    auto load_w = [&]() {
+        float one[VPT][VEC];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int j = (t + i * THREADS) * VEC;
-        if (p.w && j < p.D) load_vec<VEC>(p.w + j, w[i]);
+        for (int i = 0; i < VPT; ++i) {
+            if (p.w && i < whole) load_vec<VEC>(p.w + (t + i * THREADS) * VEC, one[i]);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            aw[i][k] = ab[i][k] = 0.0f;
-            if (!p.w || j >= p.D) w[i][k] = 1.0f;
+            for (int k = 0; k < VEC; ++k)
+                if (!p.w || i >= whole) one[i][k] = 1.0f;
         }
-    }
-    const int64_t step = (int64_t)gridDim.x * GROUPS;
-    const int64_t r0 = blockIdx.x + (int64_t)gridDim.x * group;
-    auto slot = [&](int stage, int which, int i) {
-        return ring + ((((stage * 2 + which) * VPT + i) * BT) + threadIdx.x) * VEC;
+#pragma unroll
+        for (int q = 0; q < N / 2; ++q)
+            w[q] = pair(one[2 * q / VEC][2 * q % VEC], one[(2 * q + 1) / VEC][(2 * q + 1) % VEC]);
+    };
+    constexpr bool KEEP_W = N <= 16;  // else the registers have no room for it
+    if (KEEP_W) load_w();
+#pragma unroll
+    for (int q = 0; q < N / 2; ++q) aw[q] = ab[q] = 0;
+    // Rows go to the blocks first, then to a block's warps; the lane groups of a warp take
+    // neighbouring rows and run out together.
+    constexpr int PER_WARP = THREADS < 32 ? 32 / THREADS : 1;
+    const int unit = group / PER_WARP, sub = group % PER_WARP;
+    const int64_t blocks = gridDim.x, step = blocks * GROUPS;
+    const int64_t u0 = (blockIdx.x + blocks * unit) * PER_WARP;  // first row of the warp (or group)
+    auto slot = [&](int stage, int which) { return ring + ((stage * GROUPS + group) * 2 + which) * R::ROW; };
+    auto fetch_row = [&](const float* from, float* to) {
+        if constexpr (VEC == 4) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int j = (t + i * THREADS) * 4;
+                if (i < whole) copy16(to + j, from + j);
+            }
+        } else {
+            const int phase = (int)(reinterpret_cast<uintptr_t>(from) >> 2) & 3;
+            const int pieces = (phase + p.D + 3) >> 2;
+#pragma unroll
+            for (int i = 0; i <= (VPT + 3) / 4; ++i) {
+                const int q = t + i * THREADS, j = 4 * q - phase;
+                if (j >= 0 && j + 4 <= p.D) copy16(to + 4 * q, from + j);
+            }
+            // the ends, a value a thread: before the first whole piece and behind the last
+            if (phase && t < 4 - phase && t < p.D) copy4(to + phase + t, from + t);
+            const int last = 4 * (pieces - 1) - phase;  // begin of the last piece
+            if (last + 4 > p.D && (last > 0 || !phase) && last + t < p.D && t < 4) copy4(to + phase + last + t, from + last + t);
+        }
     };
     auto fetch = [&](int64_t r, int stage) {
         if (r < p.rows) {
-            const float* xr = p.x + p.xm.offset(r);
-            const float* gr = p.g + p.gm.offset(r);
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                const int j = (t + i * THREADS) * VEC;
-                if (j < p.D) {
-                    copy_async<VEC>(slot(stage, 0, i), xr + j);
-                    copy_async<VEC>(slot(stage, 1, i), gr + j);
-                }
-            }
+            fetch_row(p.x + p.xm.offset(r), slot(stage, 0));
+            fetch_row(p.g + p.gm.offset(r), slot(stage, 1));
         }
         copies_commit();
     };
+    // where the row's values are within their slot
+    auto placed = [&](const float* from, float* at) {
+        return VEC == 4 ? at : at + ((reinterpret_cast<uintptr_t>(from) >> 2) & 3);
+    };
+    auto meet = [&]() {
+        if constexpr (THREADS <= 32)
+            __syncwarp();
+        else
+            asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(THREADS) : "memory");
+    };
 #pragma unroll
-    for (int s = 0; s < S; ++s) fetch(r0 + s * step, s);
+    for (int s = 0; s < S; ++s) fetch(u0 + s * step + sub, s);
     int stage = 0, turn = 0;
     float next[2] = {0.0f, 0.0f};
     auto fetch_stats = [&](int64_t r) {
@@ -208,61 +263,87 @@ __global__ void __launch_bounds__(BT, 1) ln_bwd_kernel(LnBwd p) {
             next[0] = st[0], next[1] = st[1];
         }
     };
-    fetch_stats(r0);
-    for (int64_t r = r0; r < p.rows; r += step) {
+    fetch_stats(u0 + sub);
+    for (int64_t u = u0; u < p.rows; u += step) {
+        const int64_t r = u + sub;
+        const bool live = PER_WARP == 1 || r < p.rows;
+        const int mine = live ? whole : 0;
         const float mean = next[0], rstd = next[1];
         fetch_stats(r + step);
         copies_wait<S - 1>();
-        float x[VPT][VEC], g[VPT][VEC];
+        if constexpr (VEC == 1) meet();
+        Pair x[N / 2], g[N / 2];
+        {
+            const float* xs = placed(p.x + (live ? p.xm.offset(r) : 0), slot(stage, 0)) + t * VEC;
+            const float* gs = placed(p.g + (live ? p.gm.offset(r) : 0), slot(stage, 1)) + t * VEC;
+            float xv[VPT][VEC], gv[VPT][VEC];
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            if ((t + i * THREADS) * VEC < p.D) {
-                load_vec<VEC>(slot(stage, 0, i), x[i]);
-                load_vec<VEC>(slot(stage, 1, i), g[i]);
-            } else {
+            for (int i = 0; i < VPT; ++i) {
+                if (i < mine) {
+                    load_vec<VEC>(xs + i * THREADS * VEC, xv[i]);
+                    load_vec<VEC>(gs + i * THREADS * VEC, gv[i]);
+                } else {  // adds nothing
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) x[i][k] = mean, g[i][k] = 0.0f;
+                    for (int k = 0; k < VEC; ++k) xv[i][k] = mean, gv[i][k] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < N / 2; ++q) {
+                x[q] = pair(xv[2 * q / VEC][2 * q % VEC], xv[(2 * q + 1) / VEC][(2 * q + 1) % VEC]);
+                g[q] = pair(gv[2 * q / VEC][2 * q % VEC], gv[(2 * q + 1) / VEC][(2 * q + 1) % VEC]);
             }
         }
-        float s[2] = {0.0f, 0.0f};
+        if (!KEEP_W) load_w();
+        const Pair shift = pair(-mean, -mean), scale = pair(rstd, rstd);
+        Pair s0 = 0, s1 = 0;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                x[i][k] = (x[i][k] - mean) * rstd;
-                aw[i][k] = fmaf(g[i][k], x[i][k], aw[i][k]);
-                ab[i][k] += g[i][k];
-                g[i][k] *= w[i][k];
-                s[0] += g[i][k];
-                s[1] = fmaf(g[i][k], x[i][k], s[1]);
-            }
+        for (int q = 0; q < N / 2; ++q) {
+            x[q] = mul2(add2(x[q], shift), scale);
+            aw[q] = fma2(g[q], x[q], aw[q]);
+            ab[q] = add2(ab[q], g[q]);
+            g[q] = mul2(g[q], w[q]);
+            s0 = add2(s0, g[q]);
+            s1 = fma2(g[q], x[q], s1);
+        }
+        if constexpr (VEC == 1) meet();
         fetch(r + S * step, stage);  // into the row just read
         stage = stage + 1 == S ? 0 : stage + 1;
         if (!p.dx) continue;
-        warp_sum(s);
+        float s[2], other[2];
+        unpair(s0, s[0], other[0]);
+        unpair(s1, s[1], other[1]);
+        s[0] += other[0], s[1] += other[1];
+        warp_sum<(THREADS < 32 ? THREADS : 32)>(s);
         if constexpr (W > 1) {
-            float* mine = red[turn][group];
-            if (lane == 0) mine[2 * (t >> 5)] = s[0], mine[2 * (t >> 5) + 1] = s[1];
-            asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(THREADS) : "memory");
+            float* sums = red[turn][group];
+            if (lane == 0) sums[2 * (t >> 5)] = s[0], sums[2 * (t >> 5) + 1] = s[1];
+            meet();
             s[0] = s[1] = 0.0f;
 #pragma unroll
-            for (int q = 0; q < W; ++q) s[0] += mine[2 * q], s[1] += mine[2 * q + 1];
+            for (int q = 0; q < W; ++q) s[0] += sums[2 * q], s[1] += sums[2 * q + 1];
             turn ^= 1;
         }
-        const float c0 = s[0] * inv, c1 = s[1] * inv;
-        float* dr = p.dx + r * p.D;
+        s[0] *= -inv, s[1] *= -inv;
+        const Pair c0 = pair(s[0], s[0]), c1 = pair(s[1], s[1]);
+        float* dr = p.dx + r * p.D + t * VEC;
+#pragma unroll
+        for (int q = 0; q < N / 2; ++q) x[q] = mul2(scale, add2(g[q], fma2(x[q], c1, c0)));
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int j = (t + i * THREADS) * VEC;
-            if (j < p.D) {
+            if (i < mine) {
                 float y[VEC], old[VEC];
-                if (p.accumulate) load_vec<VEC>(dr + j, old);
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
-                    y[k] = __fmul_rn(rstd, g[i][k] - fmaf(x[i][k], c1, c0));
-                    if (p.accumulate) y[k] = __fadd_rn(y[k], old[k]);  // the gradient rounded, then added
+                    float lo, hi;
+                    unpair(x[(i * VEC + k) / 2], lo, hi);
+                    y[k] = (i * VEC + k) % 2 ? hi : lo;
                 }
-                store_vec<VEC>(dr + j, y);
+                if (p.accumulate) {
+                    load_vec<VEC>(dr + i * THREADS * VEC, old);
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) y[k] = __fadd_rn(y[k], old[k]);  // the gradient rounded, then added
+                }
+                store_once<VEC>(dr + i * THREADS * VEC, y);
             }
         }
     }
@@ -274,16 +355,22 @@ __global__ void __launch_bounds__(BT, 1) ln_bwd_kernel(LnBwd p) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         const int j = (t + i * THREADS) * VEC;
-        if (j < p.D) {
+        if (i < whole) {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) sums[j + k] = aw[i][k], sums[p.D + j + k] = ab[i][k];
+            for (int k = 0; k < VEC; ++k) {
+                float lo, hi;
+                unpair(aw[(i * VEC + k) / 2], lo, hi);
+                sums[j + k] = (i * VEC + k) % 2 ? hi : lo;
+                unpair(ab[(i * VEC + k) / 2], lo, hi);
+                sums[p.D + j + k] = (i * VEC + k) % 2 ? hi : lo;
+            }
         }
     }
     if constexpr (GROUPS > 1) {
         __syncthreads();
         for (int j = threadIdx.x; j < 2 * p.D; j += BT) {
             float a = 0.0f;
-#pragma unroll
+#pragma unroll 8
             for (int q = 0; q < GROUPS; ++q) a += ring[q * 2 * p.D + j];
             part[j] = a;
         }
@@ -363,29 +450,24 @@ constexpr const char* kBwd = "layer_norm_backward";
 
 template <int VEC, int VPT, int THREADS>
 int launch_fwd(const LnFwd& p, cudaStream_t s) {
-    constexpr int RPB = THREADS == 32 ? 4 : 1;
+    constexpr int RPB = THREADS <= 32 ? 128 / THREADS : 1;
     const int64_t want = (p.rows + RPB - 1) / RPB;
     const unsigned grid = (unsigned)std::min<int64_t>(want, INT32_MAX);
-    ln_fwd_kernel<VEC, VPT, THREADS><<<grid, THREADS == 32 ? 128 : THREADS, 0, s>>>(p);
+    ln_fwd_kernel<VEC, VPT, THREADS><<<grid, THREADS <= 32 ? 128 : THREADS, 0, s>>>(p);
     count_launch();
     return check_launch(kFwd);
 }
 
+// 16 to 32 values a thread: many small blocks keep more rows in flight than few large ones
+// (and than rings of copies ahead: 8192 x 768 11 us, 14 through a ring).
 template <int VEC>
 int pick_fwd(const LnFwd& p, cudaStream_t s) {
     const int n = (p.D + VEC - 1) / VEC;  // vectors a row
-    if (VEC * n <= 1024) {
-        if (n <= 32) return launch_fwd<VEC, 1, 32>(p, s);
-        if (n <= 64) return launch_fwd<VEC, 2, 32>(p, s);
-        if (n <= 128) return launch_fwd<VEC, 4, 32>(p, s);
-        if (n <= 192) return launch_fwd<VEC, 6, 32>(p, s);
-        if (n <= 256) return launch_fwd<VEC, 8, 32>(p, s);
-        if constexpr (VEC == 1) {
-            if (n <= 512) return launch_fwd<VEC, 16, 32>(p, s);
-            return launch_fwd<VEC, 32, 32>(p, s);
-        }
-    }
-    // 16 to 32 values a thread: many small blocks keep more rows in flight than few large ones
+    if (p.D <= 128) return launch_fwd<VEC, 16 / VEC, 8>(p, s);
+    if (p.D <= 256) return launch_fwd<VEC, 16 / VEC, 16>(p, s);
+    if (p.D <= 512) return launch_fwd<VEC, 16 / VEC, 32>(p, s);
+    if (p.D <= 768) return launch_fwd<VEC, 24 / VEC, 32>(p, s);
+    if (p.D <= 1024) return launch_fwd<VEC, 32 / VEC, 32>(p, s);
     if constexpr (VEC == 4) {
         if (n <= 128 * 4) return launch_fwd<4, 4, 128>(p, s);
         if (n <= 256 * 4) return launch_fwd<4, 4, 256>(p, s);
@@ -405,31 +487,33 @@ int pick_fwd(const LnFwd& p, cudaStream_t s) {
     return check_launch(kFwd);
 }
 
-constexpr int kRingMax = 8192;  // 32 columns a lane of 8 warps
+constexpr int kRingMax = 16384;  // 32 columns a thread
 
-template <int VEC, int VPT, int W>
-int launch_bwd(const LnBwd& p, int grid, cudaStream_t s) {
-    const size_t ring = sizeof(float) * 2 * BT * VPT * VEC * ring_stages<VEC, VPT>();
+template <int VEC, int VPT, int THREADS>
+int launch_bwd(const LnBwd& p, int blocks, cudaStream_t s) {
+    using R = LnRing<VEC, VPT, THREADS>;
     static DeviceOnce once;
-    TLC_TRY(smem_limit_once(once, ln_bwd_kernel<VEC, VPT, W>, (int)ring));
-    ln_bwd_kernel<VEC, VPT, W><<<grid, BT, ring, s>>>(p);
+    TLC_TRY(smem_limit_once(once, ln_bwd_kernel<VEC, VPT, THREADS>, R::BYTES));
+    ln_bwd_kernel<VEC, VPT, THREADS><<<blocks, BT, R::BYTES, s>>>(p);
     count_launch();
     return check_launch(kBwd);
 }
 
-// 4 to 32 columns a lane; a row for one warp up to 1024 columns, then for 2, 4, 8.
+// 8 lanes a row up to 128 columns, the whole block from 4097 on.
 template <int VEC>
-int pick_bwd(const LnBwd& p, int grid, cudaStream_t s) {
-    if (p.D <= 128) return launch_bwd<VEC, 4 / VEC, 1>(p, grid, s);
-    if (p.D <= 256) return launch_bwd<VEC, 8 / VEC, 1>(p, grid, s);
-    if (p.D <= 512) return launch_bwd<VEC, 16 / VEC, 1>(p, grid, s);
-    if (p.D <= 768) return launch_bwd<VEC, 24 / VEC, 1>(p, grid, s);
-    if (p.D <= 1024) return launch_bwd<VEC, 32 / VEC, 1>(p, grid, s);
-    if (p.D <= 1536) return launch_bwd<VEC, 24 / VEC, 2>(p, grid, s);
-    if (p.D <= 2048) return launch_bwd<VEC, 32 / VEC, 2>(p, grid, s);
-    if (p.D <= 4096) return launch_bwd<VEC, 32 / VEC, 4>(p, grid, s);
-    if (p.D <= 6144) return launch_bwd<VEC, 24 / VEC, 8>(p, grid, s);
-    return launch_bwd<VEC, 32 / VEC, 8>(p, grid, s);
+int pick_bwd(const LnBwd& p, int blocks, cudaStream_t s) {
+    if (p.D <= 128) return launch_bwd<VEC, 16 / VEC, 8>(p, blocks, s);
+    if (p.D <= 256) return launch_bwd<VEC, 16 / VEC, 16>(p, blocks, s);
+    if (p.D <= 512) return launch_bwd<VEC, 16 / VEC, 32>(p, blocks, s);
+    if (p.D <= 768) return launch_bwd<VEC, 12 / VEC, 64>(p, blocks, s);
+    if (p.D <= 1024) return launch_bwd<VEC, 16 / VEC, 64>(p, blocks, s);
+    if (p.D <= 1536) return launch_bwd<VEC, 12 / VEC, 128>(p, blocks, s);
+    if (p.D <= 2048) return launch_bwd<VEC, 16 / VEC, 128>(p, blocks, s);
+    if (p.D <= 4096) return launch_bwd<VEC, 16 / VEC, 256>(p, blocks, s);
+    if (p.D <= 6144) return launch_bwd<VEC, 12 / VEC, 512>(p, blocks, s);
+    if (p.D <= 8192) return launch_bwd<VEC, 16 / VEC, 512>(p, blocks, s);
+    if (p.D <= 12288) return launch_bwd<VEC, 24 / VEC, 512>(p, blocks, s);
+    return launch_bwd<VEC, 32 / VEC, 512>(p, blocks, s);
 }
 
 // A weight or bias: NULL, or a 1-D tensor of length D with stride 1 (a copy in `sc` otherwise).
@@ -560,7 +644,8 @@ extern "C" int tlc_layer_norm_backward(const tlc_tensor* grad, const tlc_tensor*
     const int sms = sm_count();
     int parts = 0;
     if (p.D <= kRingMax) {
-        parts = (int)std::min<int64_t>(p.rows, sms);
+        const int rows_a_warp = p.D <= 128 ? 4 : p.D <= 256 ? 2 : 1;
+        parts = (int)std::min<int64_t>((p.rows + rows_a_warp - 1) / rows_a_warp, sms);
         if (sums) {
             TLC_TRY(scratch_alloc(&cp.p, sizeof(float) * 2 * (size_t)p.D * (size_t)parts, s));
             p.part = cp.f();

@@ -55,32 +55,6 @@ constexpr float kFloor = -160.0f;
 
 // ---- running sums ---------------------------------------------------------------------
 
-// Two floats in one 64-bit register pair: one instruction for both.
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pair(float lo, float hi) {
-    Pair p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
-    return p;
-}
-__device__ __forceinline__ void unpair(Pair p, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-    Pair d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-    Pair d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-
 // m: maximum (-inf: nothing yet), l = sum 2^y, w = sum 2^y y with y = a (x - m), a = scale log2 e.
 struct Run {
     float m = -INFINITY, l = 0.0f, w = 0.0f;

@@ -60,6 +60,26 @@ struct TokenRef {
         const int64_t o = map.offset(i);
         return wide ? static_cast<const int64_t*>(data)[o] : static_cast<int64_t>(static_cast<const int32_t*>(data)[o]);
     }
+    // The tokens first + k * step below end (-1 behind it).  All loads are issued before the first
+    // is waited for, which a loop over get() with its branches does not get from the compiler.
+    template <int N>
+    __device__ __forceinline__ void get(int64_t first, int64_t step, int64_t end, int64_t (&t)[N]) const {
+        int64_t o[N];
+        if (map.nd <= 1) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) o[k] = (first + k * step) * map.st[0];
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) o[k] = first + k * step < end ? map.offset(first + k * step) : 0;
+        }
+        if (wide) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) t[k] = first + k * step < end ? static_cast<const int64_t*>(data)[o[k]] : -1;
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) t[k] = first + k * step < end ? static_cast<const int32_t*>(data)[o[k]] : -1;
+        }
+    }
 };
 
 // ---- argument checks (host) ----------------------------------------------------------
@@ -254,31 +274,57 @@ __device__ __forceinline__ void store_once(float* p, const float (&v)[VEC]) {
         __stcs(p, v[0]);
 }
 
-// Sums of N values over a warp, in every lane.
-template <int N>
+// Two floats in one 64-bit register pair: one instruction for both.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ void unpair(Pair p, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// Sums of N values over LANES neighbouring lanes, in each of them.
+template <int LANES = 32, int N>
 __device__ __forceinline__ void warp_sum(float (&v)[N]) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int o = LANES / 2; o > 0; o >>= 1)
 #pragma unroll
         for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
 }
 
-// Sums of N values over THREADS threads (32: the warp; else the whole block),
-// in every thread.  `red` holds THREADS / 32 * N floats that nobody else uses
-// until all threads have passed one more block barrier.
+// Sums of N values over THREADS threads (at most 32: neighbouring lanes; else
+// the whole block), in every thread.  `red` holds THREADS / 32 * N floats that
+// nobody else uses until all threads have passed one more block barrier.
 template <int THREADS, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* red) {
-    warp_sum(v);
-    if constexpr (THREADS > 32) {
+    if constexpr (THREADS <= 32) {
+        warp_sum<THREADS>(v);
+    } else {
+        warp_sum(v);
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         if (lane == 0)
 #pragma unroll
             for (int n = 0; n < N; ++n) red[warp * N + n] = v[n];
         __syncthreads();
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            v[n] = lane < THREADS / 32 ? red[lane * N + n] : 0.0f;
-        }
+        for (int n = 0; n < N; ++n) v[n] = lane < THREADS / 32 ? red[lane * N + n] : 0.0f;
         warp_sum(v);
     }
 }
