@@ -1,0 +1,137 @@
+"""One training step of a small language model through the binding: embedding, layer norm,
+flash attention, Linear and token log-probabilities, forward and backward, against autograd in 64
+bits; alone, captured into a graph and replayed on other tokens, and beside an eager step."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+import tlcuda  # noqa: E402
+
+B, S, D, H, V = 3, 33, 64, 2, 203
+EMB, TEMP = 8.0, 0.9
+# Each gradient comes through at most 8 products of up to 203 terms, whose roundings (2^-24 each, of
+# random sign) add up to 8 sqrt(203) 2^-24, times what the norms and the softmax magnify them by (10).
+TOL = 8 * math.sqrt(203) * 2.0 ** -24 * 10
+
+
+def make():
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(5)
+
+    def normal(*shape, size=1.0):
+        return torch.randn(shape, generator=gen, device="cuda") * size
+
+    p = {"emb": normal(V, D, size=0.3), "w1": 1 + normal(D, size=0.2), "b1": normal(D, size=0.2),
+         "wq": normal(D, D, size=0.2), "wk": normal(D, D, size=0.2), "wv": normal(D, D, size=0.2), "bv": normal(D),
+         "w2": 1 + normal(D, size=0.2), "b2": normal(D, size=0.2), "wo": normal(D, V, size=0.3)}
+    tokens = torch.randint(0, V, (B, S + 1), generator=gen, device="cuda")
+    tokens[1, 20:] = -1  # a shorter sequence
+    return p, tokens
+
+
+def heads(x):
+    return x.view(B, S, H, D // H).transpose(1, 2).contiguous()
+
+
+def unheads(x):
+    return x.transpose(1, 2).contiguous().view(B, S, D)
+
+
+def step(p, tokens):
+    """Loss terms and gradients, as a user's program calls the operators."""
+    tl, sm = tlcuda, 1.0 / math.sqrt(D // H)
+    now, nxt = tokens[:, :-1], tokens[:, 1:]
+    h = tl.embedding(p["emb"], now, scale=EMB)
+    a, st1 = tl.layer_norm(h, p["w1"], p["b1"])
+    q, k = heads(tl.matmul(a, p["wq"])), heads(tl.matmul(a, p["wk"]))
+    v = heads(tl.matmul_fused(a, p["wv"], bias=p["bv"]))
+    o, lse = tl.flash_attention(q, k, v, sm)
+    r = tl.add_tensors(h, unheads(o))
+    y, st2 = tl.layer_norm(r, p["w2"], p["b2"])
+    logits = tl.matmul(y, p["wo"])
+    logp, ent, stats, best, which = tl.token_logprobs(logits, nxt, scale=TEMP, top=3)
+    g_lp = torch.full((), -1.0, device="cuda").expand(B, S)
+    g_ent = torch.full((), -0.1, device="cuda").expand(B, S)
+    d_logits = tl.token_logprobs_backward(logits, nxt, stats, g_lp, g_ent, ent, scale=TEMP)
+    g = {}
+    dy, g["wo"] = tl.matmul_backward(d_logits, y, p["wo"])
+    dr, g["w2"], g["b2"] = tl.layer_norm_backward(dy, r, st2, p["w2"])
+    dq, dk, dv = tl.flash_attention_backward(heads(dr), q, k, v, o, lse, sm)
+    da, g["wq"] = tl.matmul_backward(unheads(dq), a, p["wq"])
+    da, g["wk"] = tl.matmul_backward(unheads(dk), a, p["wk"], da=da, db=torch.zeros_like(p["wk"]), accumulate=True)
+    da, g["wv"] = tl.matmul_backward(unheads(dv), a, p["wv"], da=da, db=torch.zeros_like(p["wv"]), accumulate=True)
+    g["bv"] = tl.sum_to(unheads(dv), (D,))
+    # the residual branch's gradient is in dr already: the norm's is added to it
+    dh, g["w1"], g["b1"] = tl.layer_norm_backward(da, h, st1, p["w1"], dx=dr, dweight=torch.zeros_like(p["w1"]),
+                                                  dbias=torch.zeros_like(p["b1"]), accumulate=True)
+    g["emb"] = tl.embedding_backward(dh, now, V, scale=EMB)
+    return (logp, ent, best, which), g
+
+
+def reference(p, tokens):
+    q = {k: v.double().requires_grad_() for k, v in p.items()}
+    now, nxt = tokens[:, :-1], tokens[:, 1:]
+    h = torch.where((now >= 0).unsqueeze(-1), q["emb"][now.clamp(min=0)] * EMB, 0.0)
+
+    def norm(x, w, b):
+        m = x.mean(-1, keepdim=True)
+        return (x - m) / torch.sqrt(((x - m) ** 2).mean(-1, keepdim=True) + 1e-5) * w + b
+
+    a = norm(h, q["w1"], q["b1"])
+
+    def split(x):
+        return x.view(B, S, H, D // H).transpose(1, 2)
+
+    s = split(a @ q["wq"]) @ split(a @ q["wk"]).transpose(-1, -2) / math.sqrt(D // H)
+    o = torch.softmax(s, -1) @ split(a @ q["wv"] + q["bv"])
+    r = h + o.transpose(1, 2).reshape(B, S, D)
+    logits = norm(r, q["w2"], q["b2"]) @ q["wo"]
+    every = torch.log_softmax(logits * float(torch.tensor(TEMP)), -1)
+    logp = torch.where(nxt >= 0, every.gather(-1, nxt.clamp(min=0).unsqueeze(-1))[..., 0], 0.0)
+    ent = -(every.exp() * every).sum(-1)
+    (-logp.sum() - 0.1 * ent.sum()).backward()
+    best = every.topk(3, -1)
+    return (logp, ent, best.values, best.indices), {k: v.grad for k, v in q.items()}
+
+
+def check(got, want):
+    for i, (a, b) in enumerate(zip(got[0], want[0])):
+        if i == 3:
+            assert torch.equal(a, b)
+        else:
+            assert float((a.double() - b).norm() / b.norm()) <= TOL, i
+    for k, b in want[1].items():
+        assert float((got[1][k].double() - b).norm() / b.norm()) <= TOL, k
+
+
+def test_training_step():
+    p, tokens = make()
+    check(step(p, tokens), reference(p, tokens))
+
+
+def test_training_step_in_a_graph():
+    p, tokens = make()
+    eager = step(p, tokens)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = step(p, tokens)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip((*out[0], *out[1].values()), (*eager[0], *eager[1].values())):
+        assert torch.equal(a, b)
+    # other tokens in the same memory, replayed while an eager step runs on another stream
+    other = torch.roll(tokens, 1, 0).flip(1).contiguous()
+    other[0, :3] = -1
+    tokens.copy_(other)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        graph.replay()
+    again = step(p, other)
+    torch.cuda.synchronize()
+    check(out, reference(p, other))
+    check(again, reference(p, other))

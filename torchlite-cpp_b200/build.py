@@ -2,7 +2,8 @@
 
   lib/libtl_cuda.so         CUDA kernels + the C ABI (include/tlc.h), sm_100a only
   lib/libtorchlite_b200.so  the C++ tl:: layer (host/) over the C ABI
-  lib/tl_tests              C++ tests of the tl:: layer (host/tests)
+  lib/tl_tests              C++ tests of the tl:: layer (host/tests/test_matmul.cpp)
+  lib/tl_token_tests        C++ tests of its token-model ops (host/tests/test_tokens.cpp)
 
 Usage:  python torchlite-cpp_b200/build.py [--jobs N] [--verbose]
 """
@@ -73,11 +74,12 @@ def build(jobs: int = 8, verbose: bool = False, ptxas_info: bool = False) -> dic
     if host_src and _stale(tl_so, host_src + host_hdr + [so]):
         _run(["g++"] + CXX_FLAGS + ["-shared", "-o", tl_so] + host_src +
              ["-L", LIB, "-ltl_cuda", "-Wl,-rpath,$ORIGIN"], verbose)
-    test_src = sorted(glob.glob(os.path.join(PKG, "host", "tests", "*.cpp")))
-    test_bin = os.path.join(LIB, "tl_tests")
-    if test_src and _stale(test_bin, test_src + host_hdr + [tl_so]):
-        _run(["g++"] + CXX_FLAGS + ["-UNDEBUG", "-o", test_bin] + test_src +
-             ["-L", LIB, "-ltorchlite_b200", "-ltl_cuda", "-Wl,-rpath,$ORIGIN"], verbose)
+    for src, name in (("test_matmul.cpp", "tl_tests"), ("test_tokens.cpp", "tl_token_tests")):
+        test_src = os.path.join(PKG, "host", "tests", src)
+        test_bin = os.path.join(LIB, name)
+        if os.path.exists(test_src) and _stale(test_bin, [test_src] + host_hdr + [tl_so]):
+            _run(["g++"] + CXX_FLAGS + ["-UNDEBUG", "-o", test_bin, test_src,
+                  "-L", LIB, "-ltorchlite_b200", "-ltl_cuda", "-Wl,-rpath,$ORIGIN"], verbose)
     # The reference callers' scenarios on the device tl:: layer
     # (tests/integration/device_callers_main.cpp, compared with the reference
     # by tests/test_reference_callers.py).

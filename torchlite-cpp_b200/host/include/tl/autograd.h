@@ -5,6 +5,7 @@
 #pragma once
 
 #include <tl/tensor.h>
+#include <tl/tokens.h>
 
 #include <cstdint>
 #include <initializer_list>
@@ -101,6 +102,32 @@ class FusedMatmulBackward : public GradFunction {
     float scalar = 1.0f;
     bool apply_scale = false;
     int mode = -1;
+    void backward(const Tensor& grad_output) override;
+};
+
+// Layer norm (inputs: x, weight, bias; the latter two may be empty).
+class LayerNormBackward : public GradFunction {
+  public:
+    Tensor x_cache, weight_cache, stats_cache;
+    void backward(const Tensor& grad_output) override;
+};
+
+// The table's gradient: sums over the positions of each token (inputs: weight).
+class EmbeddingBackward : public GradFunction {
+  public:
+    Tokens tokens;
+    std::vector<int64_t> weight_sizes;
+    float scale = 1.0f;
+    void backward(const Tensor& grad_output) override;
+};
+
+// token_logprobs' gradient to the logits, from log p or from the entropy.
+class TokenLogprobsBackward : public GradFunction {
+  public:
+    Tensor logits_cache, stats_cache, entropy_cache;
+    Tokens tokens;
+    float scale = 1.0f;
+    bool of_entropy = false;
     void backward(const Tensor& grad_output) override;
 };
 

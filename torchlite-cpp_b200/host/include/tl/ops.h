@@ -2,6 +2,7 @@
 #pragma once
 
 #include <tl/tensor.h>
+#include <tl/tokens.h>
 
 #include <cstdint>
 #include <vector>
@@ -63,6 +64,22 @@ Tensor conv2d(const Tensor& input, const Tensor& weight, const Tensor& bias, int
 // softmax; FlashAttentionBackward in the process default GEMM mode.  Agrees
 // with the reference to its own 1e-4 bar (CUDA's expf / logf).
 Tensor flash_attention(const Tensor& Q, const Tensor& K, const Tensor& V, float sm_scale);
+// Layer norm over the last dim (nn::LayerNorm of the reference, nn.h:56-630):
+// (x - mean) / sqrt(var + eps) * weight + bias, weight and bias [D] or empty.
+// The row's mean and 1 / sqrt(var + eps) are kept for the gradient.
+Tensor layer_norm(const Tensor& input, const Tensor& weight, const Tensor& bias, float eps = 1e-5f);
+// scale * weight[tokens] (nn::Embedding): [tokens' shape, D]; token -1 gives
+// zeros and no gradient, any other token outside the table a row of NaN.
+Tensor embedding(const Tensor& weight, const Tokens& tokens, float scale = 1.0f);
+// What softmax(scale * logits) over the last dim says of the tokens (one a row):
+// log p of each (0 for token -1), the entropy of each row, and the `top` <= 32
+// most likely tokens with their log p.  logprobs and entropy carry gradients
+// to the logits (the mean of -logprobs is the cross-entropy, loss.cpp:12-103).
+struct TokenScores {
+    Tensor logprobs, entropy, top_logprobs;
+    Tokens top_tokens;
+};
+TokenScores token_logprobs(const Tensor& logits, const Tokens& tokens, float scale = 1.0f, int top = 0);
 // sum along a dimension (src/ops.cpp:1181-1233); no autograd node
 Tensor sum(const Tensor& input, int64_t dim, bool keepdim = false);
 

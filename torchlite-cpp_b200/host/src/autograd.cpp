@@ -39,6 +39,20 @@ tlc_tensor hview(const Tensor& t) {
     return v;
 }
 
+tlc_index iview(const Tokens& t) {
+    tlc_index v{};
+    v.ndim = static_cast<int32_t>(t.sizes().size());
+    v.bits = 64;
+    int64_t step = 1;
+    for (int i = v.ndim - 1; i >= 0; --i) {
+        v.sizes[i] = t.sizes()[i];
+        v.strides[i] = step;
+        step *= t.sizes()[i];
+    }
+    v.data = t.numel() > 0 ? const_cast<int64_t*>(t.device_data()) : nullptr;
+    return v;
+}
+
 }  // namespace
 
 // src/autograd.cpp:16-22: the first gradient is zeros + d, later ones add.
@@ -192,6 +206,57 @@ void FusedMatmulBackward::backward(const Tensor& grad_output) {
     mm.squeeze_b = b_cache.sizes().size() == 1;
     mm.mode = mode;
     mm.backward(g);
+}
+
+void LayerNormBackward::backward(const Tensor& grad_output) {
+    const bool want_x = inputs[0].requires_grad;
+    const bool want_w = inputs[1].requires_grad && !inputs[1].empty();
+    const bool want_b = inputs[2].requires_grad && !inputs[2].empty();
+    if (!want_x && !want_w && !want_b) return;
+    const std::vector<int64_t> cols = {x_cache.sizes().back()};
+    Tensor dx, dw, db;
+    tlc_tensor vdx{}, vdw{}, vdb{}, vw{};
+    if (want_x) {
+        dx = Tensor::device_empty(x_cache.sizes());
+        vdx = dview(dx);
+    }
+    if (want_w) {
+        dw = Tensor::device_empty(cols);
+        vdw = dview(dw);
+    }
+    if (want_b) {
+        db = Tensor::device_empty(cols);
+        vdb = dview(db);
+    }
+    if (!weight_cache.empty()) vw = dview(weight_cache);
+    tlc_tensor g = dview(grad_output), x = dview(x_cache), st = dview(stats_cache);
+    check(tlc_layer_norm_backward(&g, &x, &st, weight_cache.empty() ? nullptr : &vw, want_x ? &vdx : nullptr,
+                                  want_w ? &vdw : nullptr, want_b ? &vdb : nullptr, 0, nullptr),
+          "tlc_layer_norm_backward");
+    if (want_x) accumulate_grad(inputs[0], dx);
+    if (want_w) accumulate_grad(inputs[1], dw);
+    if (want_b) accumulate_grad(inputs[2], db);
+}
+
+void EmbeddingBackward::backward(const Tensor& grad_output) {
+    if (!inputs[0].requires_grad) return;
+    Tensor dw = Tensor::device_empty(weight_sizes);
+    tlc_tensor g = dview(grad_output), vd = dview(dw);
+    tlc_index t = iview(tokens);
+    check(tlc_embedding_backward(&g, &t, scale, &vd, 0, nullptr), "tlc_embedding_backward");
+    accumulate_grad(inputs[0], dw);
+}
+
+void TokenLogprobsBackward::backward(const Tensor& grad_output) {
+    if (!inputs[0].requires_grad) return;
+    Tensor dx = Tensor::device_empty(logits_cache.sizes());
+    tlc_tensor x = dview(logits_cache), st = dview(stats_cache), g = dview(grad_output), vd = dview(dx), h{};
+    if (of_entropy) h = dview(entropy_cache);
+    tlc_index t = iview(tokens);
+    check(tlc_token_logprobs_backward(&x, &t, &st, of_entropy ? &h : nullptr, of_entropy ? nullptr : &g,
+                                      of_entropy ? &g : nullptr, scale, &vd, nullptr),
+          "tlc_token_logprobs_backward");
+    accumulate_grad(inputs[0], dx);
 }
 
 }  // namespace tl

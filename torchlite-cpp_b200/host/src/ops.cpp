@@ -362,6 +362,113 @@ Tensor flash_attention(const Tensor& Q, const Tensor& K, const Tensor& V, float 
     return O;
 }
 
+namespace {
+
+tlc_index index_of(const Tokens& t) {
+    if (t.empty()) throw std::invalid_argument("Tokens: empty");
+    if (t.sizes().size() > TLC_MAX_DIMS) throw std::invalid_argument("Tokens: more than 8 dims");
+    tlc_index v{};
+    v.ndim = static_cast<int32_t>(t.sizes().size());
+    v.bits = 64;
+    int64_t step = 1;
+    for (int i = v.ndim - 1; i >= 0; --i) {
+        v.sizes[i] = t.sizes()[i];
+        v.strides[i] = step;
+        step *= t.sizes()[i];
+    }
+    v.data = t.numel() > 0 ? const_cast<int64_t*>(t.device_data()) : nullptr;
+    return v;
+}
+
+// The view of a result that the call writes on the device.
+tlc_tensor out_view(Tensor& t) {
+    tlc_tensor v = view_of(t, false);
+    if (t.numel() > 0) v.data = t.device_data();
+    return v;
+}
+
+}  // namespace
+
+Tensor layer_norm(const Tensor& input, const Tensor& weight, const Tensor& bias, float eps) {
+    if (input.sizes().empty()) throw std::invalid_argument("layer_norm: x must be at least 1-D");
+    std::vector<int64_t> rows = input.sizes();
+    rows.back() = 2;
+    Tensor out = Tensor::device_empty(input.sizes()), stats = Tensor::device_empty(rows);
+    tlc_tensor vx = view_of(input, true), vw{}, vb{}, vo = out_view(out), vs = out_view(stats);
+    if (!weight.empty()) vw = view_of(weight, true);
+    if (!bias.empty()) vb = view_of(bias, true);
+    check(tlc_layer_norm(&vx, weight.empty() ? nullptr : &vw, bias.empty() ? nullptr : &vb, eps, &vo, &vs, nullptr),
+          "tlc_layer_norm");
+    if (input.requires_grad || weight.requires_grad || bias.requires_grad) {
+        if (auto fn = track<LayerNormBackward>(out, {&input, &weight, &bias})) {
+            fn->x_cache = input;
+            fn->weight_cache = weight;
+            fn->stats_cache = stats;
+        }
+    }
+    return out;
+}
+
+Tensor embedding(const Tensor& weight, const Tokens& tokens, float scale) {
+    if (weight.sizes().size() != 2) throw std::invalid_argument("embedding: weight must be 2-D");
+    tlc_index vt = index_of(tokens);
+    std::vector<int64_t> sizes = tokens.sizes();
+    sizes.push_back(weight.sizes()[1]);
+    if (sizes.size() > TLC_MAX_DIMS) throw std::invalid_argument("embedding: tokens have too many dims");
+    Tensor out = Tensor::device_empty(sizes);
+    tlc_tensor vw = view_of(weight, true), vo = out_view(out);
+    check(tlc_embedding(&vw, &vt, scale, &vo, nullptr), "tlc_embedding");
+    if (weight.requires_grad) {
+        if (auto fn = track<EmbeddingBackward>(out, {&weight})) {
+            fn->tokens = tokens;
+            fn->weight_sizes = weight.sizes();
+            fn->scale = scale;
+        }
+    }
+    return out;
+}
+
+TokenScores token_logprobs(const Tensor& logits, const Tokens& tokens, float scale, int top) {
+    if (logits.sizes().empty()) throw std::invalid_argument("token_logprobs: logits must be at least 1-D");
+    if (top < 0) throw std::invalid_argument("token_logprobs: top must be 0 to the vocabulary's size");
+    const std::vector<int64_t> lead(logits.sizes().begin(), logits.sizes().end() - 1);
+    auto with = [&](int64_t n) {
+        std::vector<int64_t> s = lead;
+        s.push_back(n);
+        return s;
+    };
+    tlc_index vt = index_of(tokens), vi{};
+    TokenScores r;
+    r.logprobs = Tensor::device_empty(lead);
+    r.entropy = Tensor::device_empty(lead);
+    Tensor stats = Tensor::device_empty(with(2));
+    tlc_tensor vx = view_of(logits, true), vl = out_view(r.logprobs), ve = out_view(r.entropy), vs = out_view(stats);
+    tlc_tensor vp{};
+    if (top > 0) {
+        r.top_logprobs = Tensor::device_empty(with(top));
+        r.top_tokens = Tokens::device_empty(with(top));
+        vp = out_view(r.top_logprobs);
+        r.top_tokens.device_out();
+        vi = index_of(r.top_tokens);
+    }
+    check(tlc_token_logprobs(&vx, &vt, scale, &vl, &ve, &vs, top, top > 0 ? &vp : nullptr, top > 0 ? &vi : nullptr,
+                             nullptr),
+          "tlc_token_logprobs");
+    if (logits.requires_grad) {
+        for (Tensor* out : {&r.logprobs, &r.entropy}) {
+            if (auto fn = track<TokenLogprobsBackward>(*out, {&logits})) {
+                fn->logits_cache = logits;
+                fn->stats_cache = stats;
+                fn->tokens = tokens;
+                fn->scale = scale;
+                fn->of_entropy = out == &r.entropy;
+                if (fn->of_entropy) fn->entropy_cache = detached(r.entropy);
+            }
+        }
+    }
+    return r;
+}
+
 Tensor sum(const Tensor& input, int64_t dim, bool keepdim) {
     Tensor a = input.contiguous();
     const auto& sizes = a.sizes();
