@@ -25,6 +25,7 @@
 // token outside [0, V) gives NaN.
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 #include "rows.cuh"
 #include "tcgen05.cuh"
@@ -50,6 +51,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
+// The largest of three, NaN if one is; the smallest of three numbers.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float y;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
 // Exponents below this give 0; the bound keeps 0 * exponent from being NaN.
 constexpr float kFloor = -160.0f;
 
@@ -69,18 +81,9 @@ struct Run {
         l *= c;
         m = to;
     }
-    __device__ __forceinline__ void merge(const Run& o, float a) {
-        const float to = max_nan(m, o.m);
-        Run q = o;
-        if (m != to) raise(to, a);
-        if (q.m != to) q.raise(to, a);
-        l += q.l;
-        w += q.w;
-        m = to;
-    }
 };
 
-// Adds values to a run, two at a time: 9 instructions for two values.
+// Adds values to a run, two at a time: 8 instructions for two values.
 struct PairRun {
     float m = -INFINITY;
     // batch `where` has m, batch `where2` the second largest of the batches' maxima, `rest` is the
@@ -92,9 +95,13 @@ struct PairRun {
     __device__ __forceinline__ explicit PairRun(float scale2) : l(0), w(0), a2(pair(scale2, scale2)), a(scale2) {}
     template <int N>
     __device__ __forceinline__ void add(const float (&v)[N], int batch) {
-        float top = v[0];
+        float top = v[0], low = v[0];
 #pragma unroll
-        for (int i = 1; i < N; ++i) top = max_nan(top, v[i]);
+        for (int i = 1; i < N; i += 2) {
+            const float other = i + 1 < N ? v[i + 1] : v[i];
+            top = max3_nan(top, v[i], other);
+            low = min3(low, v[i], other);
+        }
         if (!(top <= m)) {  // also when top is NaN
             const float to = max_nan(top, m);
             if (m != -INFINITY) {
@@ -113,15 +120,26 @@ struct PairRun {
         }
         const float base = m == -INFINITY ? 0.0f : -m;
         const Pair shift = pair(base, base);
+        // masked values need the bound on their exponent; without any it is left out
+        if ((low + base) * a >= kFloor)
+            exponentials<N, false>(v, shift);
+        else
+            exponentials<N, true>(v, shift);
+    }
+    template <int N, bool BOUND>
+    __device__ __forceinline__ void exponentials(const float (&v)[N], Pair shift) {
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
-            const Pair y2 = mul2(add2(pair(v[i], i + 1 < N ? v[i + 1] : -INFINITY), shift), a2);
+            Pair y2 = mul2(add2(pair(v[i], i + 1 < N ? v[i + 1] : -INFINITY), shift), a2);
             float y0, y1;
             unpair(y2, y0, y1);
-            y0 = max_nan(y0, kFloor), y1 = max_nan(y1, kFloor);
+            if (BOUND || i + 1 == N) {
+                y0 = max_nan(y0, kFloor), y1 = max_nan(y1, kFloor);
+                y2 = pair(y0, y1);
+            }
             const Pair e = pair(ex2(y0), ex2(y1));
             l = add2(l, e);
-            w = fma2(e, pair(y0, y1), w);
+            w = fma2(e, y2, w);
         }
     }
     __device__ __forceinline__ Run sum() const {
@@ -136,15 +154,16 @@ struct PairRun {
     }
 };
 
+// The runs of a warp's lanes as one, in every lane: all are raised to the common
+// maximum first, then only sums are left.
 __device__ __forceinline__ Run warp_run(Run r, float a) {
+    float to = r.m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Run q;
-        q.m = __shfl_xor_sync(0xffffffffu, r.m, o);
-        q.l = __shfl_xor_sync(0xffffffffu, r.l, o);
-        q.w = __shfl_xor_sync(0xffffffffu, r.w, o);
-        r.merge(q, a);
-    }
+    for (int o = 16; o > 0; o >>= 1) to = max_nan(to, __shfl_xor_sync(0xffffffffu, to, o));
+    if (r.m != to) r.raise(to, a);
+    float s[2] = {r.l, r.w};
+    warp_sum(s);
+    r.m = to, r.l = s[0], r.w = s[1];
     return r;
 }
 
@@ -163,6 +182,20 @@ __device__ __forceinline__ uint32_t index_of(uint64_t key) { return ~(uint32_t)k
 __device__ __forceinline__ float value_of(uint64_t key) {
     const uint32_t u = (uint32_t)(key >> 32);
     return u == 0xffffffffu ? __int_as_float(0x7fc00000) : __uint_as_float((u & 0x80000000u) ? u ^ 0x80000000u : ~u);
+}
+
+// The highest bound that k of a warp's values (some a lane) reach, to its first
+// 16 bits: sign, exponent, 7 of the mantissa.
+template <class... V>
+__device__ __forceinline__ uint32_t highest_bound(int k, V... v) {
+    uint32_t bound = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t to = bound | (1u << bit);
+        const int reach = (__popc(__ballot_sync(0xffffffffu, v >= to)) + ...);
+        if (reach >= k) bound = to;
+    }
+    return bound;
 }
 
 struct LpFwd {
@@ -253,41 +286,57 @@ struct Part {
 
 // The values of a thread's rows, batch by batch, through a ring of asynchronous
 // copies that runs across the rows' ends, so that the memory stays busy while a
-// row's results are put together.  T threads share a row; a thread copies what
-// it reads itself, which needs no barrier.
+// row's results are put together.  T threads of a 256-thread block share a row;
+// a thread copies what it reads itself, which needs no barrier.  Whole batches,
+// nearly all of them, go without tests of single vectors.
 template <int T>
 struct Feed {
-    float4* ring;  // [STAGES][BATCH], this thread's float4 `pitch` apart
-    int pitch, t;
+    static constexpr int STEP = BATCH * T;  // vectors of a batch
+    float4* ring;                           // [STAGES][BATCH][256], this thread's
+    int t;
     const LpFwd& p;
     int lo, hi;
     int64_t row, step;
-    int at = 0, stage = 0;
-    Part part;
-    __device__ __forceinline__ Feed(float4* ring_, int pitch_, int t_, const LpFwd& p_, int lo_, int hi_, int64_t first,
-                                    int64_t step_)
-        : ring(ring_), pitch(pitch_), t(t_), p(p_), lo(lo_), hi(hi_), row(first), step(step_),
-          part(p_.x + (first < p_.rows ? p_.xm.offset(first) : 0), lo_, hi_) {
+    const float4* src = nullptr;  // this thread's next vector of the row being copied
+    int left = 0;                 // vectors of that row, from thread 0's next one on
+    int stage = 0;
+    __device__ __forceinline__ Feed(float4* ring_, int t_, const LpFwd& p_, int lo_, int hi_, int64_t first, int64_t step_)
+        : ring(ring_), t(t_), p(p_), lo(lo_), hi(hi_), row(first), step(step_) {
+        open();
 #pragma unroll
         for (int q = 0; q < STAGES; ++q) fetch(q);
     }
+    template <int... U>
+    __device__ __forceinline__ void copy_batch(uint32_t to, const float4* from, std::integer_sequence<int, U...>) {
+        (copy_at<U * 256 * 16, U * T * 16>(to, from), ...);
+    }
+    template <int TO, int FROM>
+    __device__ __forceinline__ void copy_at(uint32_t to, const float4* from) {
+        asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(to), "l"(from), "n"(TO), "n"(FROM) : "memory");
+    }
+    __device__ __forceinline__ void open() {
+        if (row >= p.rows) return;
+        const Part part(p.x + p.xm.offset(row), lo, hi);
+        src = reinterpret_cast<const float4*>(part.x + part.head) + t;
+        left = part.vecs;
+    }
     __device__ __forceinline__ void fetch(int to) {
         if (row < p.rows) {
-            const float4* from = reinterpret_cast<const float4*>(part.x + part.head);
+            const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(ring + to * BATCH * 256));
+            if (left >= STEP) {
+                copy_batch(at, src, std::make_integer_sequence<int, BATCH>());
+            } else {
 #pragma unroll
-            for (int u = 0; u < BATCH; ++u) {
-                const int i = at + t + u * T;
-                if (i < part.vecs)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
-                                     __cvta_generic_to_shared(ring + (to * BATCH + u) * pitch))),
-                                 "l"(from + i)
-                                 : "memory");
+                for (int u = 0; u < BATCH; ++u)
+                    if (t + u * T < left)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + u * 256 * 16), "l"(src + u * T)
+                                     : "memory");
             }
-            at += BATCH * T;
-            if (at >= part.vecs) {  // every row has one batch at least
-                at = 0;
+            src += STEP;
+            left -= STEP;
+            if (left <= 0) {  // every row has one batch at least
                 row += step;
-                if (row < p.rows) part = Part(p.x + p.xm.offset(row), lo, hi);
+                open();
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -296,21 +345,31 @@ struct Feed {
     __device__ __forceinline__ void add_row(const Part& now, PairRun& own) {
         const int alone_at = now.single(t);
         const float alone = alone_at >= 0 ? now.x[alone_at] : -INFINITY;
-        int batch = 0;
+        int batch = 0, rest = now.vecs;
         do {
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
             float v[4 * BATCH];
+            const float4* from = ring + stage * BATCH * 256;
+            if (rest >= STEP) {
 #pragma unroll
-            for (int u = 0; u < BATCH; ++u) {
-                float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if ((batch * BATCH + u) * T + t < now.vecs) f = ring[(stage * BATCH + u) * pitch];
-                v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
+                for (int u = 0; u < BATCH; ++u) {
+                    const float4 f = from[u * 256];
+                    v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < BATCH; ++u) {
+                    float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (t + u * T < rest) f = from[u * 256];
+                    v[4 * u] = f.x, v[4 * u + 1] = f.y, v[4 * u + 2] = f.z, v[4 * u + 3] = f.w;
+                }
             }
             fetch(stage);  // into what was just read
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             own.add(v, batch);
             ++batch;
-        } while (batch * BATCH * T < now.vecs);
+            rest -= STEP;
+        } while (rest > 0);
         if (alone_at >= 0) {
             const float v[1] = {alone};
             own.add(v, -1);
@@ -365,7 +424,6 @@ __device__ __forceinline__ void look_together(const Part& part, int t, int begin
 // ---- a row for a warp -------------------------------------------------------------------
 
 constexpr int WARP_CAP = 128;  // candidates for the alternatives that a warp keeps
-constexpr int BOUND_BITS = 16;  // of a bound's 32: sign, exponent, 7 of the mantissa
 
 // A warp a row, 8 rows a block at once.
 template <bool TOP>
@@ -375,7 +433,7 @@ __global__ void __launch_bounds__(256, 3) lp_warp_kernel(LpFwd p) {
     __shared__ int founds[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t first = blockIdx.x + (int64_t)gridDim.x * warp, step = (int64_t)gridDim.x * 8;
-    Feed<32> feed(ring + threadIdx.x, 256, lane, p, 0, p.V, first, step);
+    Feed<32> feed(ring + threadIdx.x, lane, p, 0, p.V, first, step);
     for (int64_t r = first; r < p.rows; r += step) {
         const float* x = p.x + p.xm.offset(r);
         const Part part(x, 0, p.V);
@@ -390,17 +448,9 @@ __global__ void __launch_bounds__(256, 3) lp_warp_kernel(LpFwd p) {
             int found = WARP_CAP + 1;
             if (s.m == s.m) {
                 // Each lane has three maxima of disjoint sets of its values.  What `top` of
-                // these 96 reach, `top` values reach: the highest such bound, bit by bit.
+                // these 96 reach, `top` values reach.
                 const uint32_t most = order_of(own.m), second = order_of(own.second), rest = order_of(own.rest);
-                uint32_t bound = 0;
-#pragma unroll
-                for (int bit = 31; bit >= 32 - BOUND_BITS; --bit) {
-                    const uint32_t to = bound | (1u << bit);
-                    const int reach = __popc(__ballot_sync(0xffffffffu, most >= to)) +
-                                      __popc(__ballot_sync(0xffffffffu, second >= to)) +
-                                      __popc(__ballot_sync(0xffffffffu, rest >= to));
-                    if (reach >= p.top) bound = to;
-                }
+                const uint32_t bound = highest_bound(p.top, most, second, rest);
                 if (lane == 0) founds[warp] = 0;
                 __syncwarp();
                 auto take = [&](float v, int at) {
@@ -483,14 +533,9 @@ __device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top, floa
     if (tid == 0) sm.threads = sm.found = 0;
     if (tid < kMaxTop) sm.best[tid] = 0;
     __syncthreads();
-    if (tid < 64) {  // the k-th largest of the groups' maxima
-        const uint32_t v = sm.group[tid];
-        int above = 0;
-        for (int j = 0; j < 64; ++j) {
-            const uint32_t o = sm.group[j];
-            above += o > v || (o == v && j < tid);
-        }
-        if (above == k - 1) sm.bound = v;
+    if (warp == 0) {
+        const uint32_t reach = highest_bound(k, sm.group[lane], sm.group[lane + 32]);
+        if (lane == 0) sm.bound = reach;
     }
     __syncthreads();
     const uint32_t bound = sm.bound;
@@ -579,7 +624,8 @@ __global__ void __launch_bounds__(T) lp_row_kernel(LpFwd p, int C) {
     const int per = ((p.V + C - 1) / C + 31) & ~31;
     const int lo = (int)min((int64_t)p.V, (int64_t)rank * per), hi = (int)min((int64_t)p.V, (int64_t)lo + per);
 
-    Feed<T> feed(ring + tid, T, tid, p, lo, hi, first, step);
+    static_assert(T == 256, "the ring's layout");
+    Feed<T> feed(ring + tid, tid, p, lo, hi, first, step);
     for (int64_t r = first; r < p.rows; r += step) {
         const float* x = p.x + p.xm.offset(r);
         const Part part(x, lo, hi);
