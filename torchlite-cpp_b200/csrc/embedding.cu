@@ -320,6 +320,7 @@ __device__ void fill_absent(const SortArgs& p, FillSmem& sm, uint32_t cluster, u
 
 __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(SORT_T) embed_sort_kernel(SortArgs p) {
     extern __shared__ __align__(16) unsigned char raw[];
+    next_may_launch();
     const int cluster = (int)blockIdx.x / CL, clusters = (int)gridDim.x / CL;
     if (cluster == 0)
         sort_positions(p, *reinterpret_cast<SortSmem*>(raw));
@@ -362,6 +363,8 @@ __device__ __forceinline__ void write_row(const SumArgs& p, int64_t row, int j, 
 // position's key and row; where runs end is one mask.
 template <int VEC, int VPT>
 __global__ void __launch_bounds__(256) embed_sum_kernel(SumArgs p, int64_t units, int slices) {
+    next_may_launch();
+    after_previous();
     const int lane = threadIdx.x & 31;
     const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (u >= units) return;
@@ -451,6 +454,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(SumArgs p, int slices) 
     __shared__ int long_chunk[8], long_slice[8], long_count[8];
     __shared__ float eighth[8][32 * VEC];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    after_previous();
     const int runs = *p.crossing;
     const int64_t units = (int64_t)runs * slices;
     // the block's warps take units far apart: frequent tokens, neighbours in the list, have long runs
@@ -547,15 +551,12 @@ int launch_sums(const SumArgs& p, cudaStream_t s) {
     const int slices = (p.D + 32 * VEC * VPT - 1) / (32 * VEC * VPT);
     const int64_t blocks = (chunks * slices + 7) / 8;
     if (blocks > INT32_MAX) return set_error(TLC_ERR_UNSUPPORTED, "embedding_backward: too many tokens");
-    embed_sum_kernel<VEC, VPT><<<(unsigned)blocks, 256, 0, s>>>(p, chunks * slices, slices);
-    count_launch();
-    TLC_TRY(check_launch(kBwd));
+    TLC_TRY(launch_after(embed_sum_kernel<VEC, VPT>, (unsigned)blocks, 256, s, kBwd, p, chunks * slices, slices));
     if (chunks == 1) return TLC_OK;  // no run crosses
     // the number of crossing runs is on the device: enough blocks to keep every SM busy
     const int thin = (p.D + 32 * VEC - 1) / (32 * VEC);
-    embed_join_kernel<VEC><<<(unsigned)std::min<int64_t>((chunks * thin + 7) / 8, 148 * 4), 256, 0, s>>>(p, thin);
-    count_launch();
-    return check_launch(kBwd);
+    const unsigned grid = (unsigned)std::min<int64_t>((chunks * thin + 7) / 8, (int64_t)sm_count() * 4);
+    return launch_after(embed_join_kernel<VEC>, grid, 256, s, kBwd, p, thin);
 }
 
 // The most clusters of the sort kernel that run at once on the current device.

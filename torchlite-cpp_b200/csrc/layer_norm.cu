@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(BT, 1) ln_bwd_kernel(LnBwd p) {
     __shared__ float red[2][GROUPS][2 * W];
     const int group = threadIdx.x / THREADS, t = threadIdx.x % THREADS, lane = threadIdx.x & 31;
     const float inv = 1.0f / (float)p.D;
+    next_may_launch();
     const int vecs = p.D / VEC;
     const int whole = vecs / THREADS + (t < vecs % THREADS ? 1 : 0);  // this thread's vectors of a row
     Pair aw[N / 2], ab[N / 2], w[N / 2];
@@ -428,6 +429,7 @@ __global__ void __launch_bounds__(256) ln_bwd_cols_kernel(LnBwd p, int64_t rows_
 __global__ void __launch_bounds__(512) ln_bwd_finish_kernel(const float* __restrict__ part, int parts, int D,
                                                             float* dw, float* db, int accumulate) {
     __shared__ float red[16][33];
+    after_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t j = (int64_t)blockIdx.x * 32 + lane;
     float a = 0.0f;
@@ -671,10 +673,8 @@ extern "C" int tlc_layer_norm_backward(const tlc_tensor* grad, const tlc_tensor*
     }
     if (sums) {
         const int64_t blocks = (2 * (int64_t)p.D + 31) / 32;
-        ln_bwd_finish_kernel<<<(unsigned)blocks, 512, 0, s>>>(p.part, parts, p.D, dweight ? dweight->data : nullptr,
-                                                             dbias ? dbias->data : nullptr, p.accumulate);
-        count_launch();
-        TLC_TRY(check_launch(kBwd));
+        TLC_TRY(launch_after(ln_bwd_finish_kernel, (unsigned)blocks, 512, s, kBwd, (const float*)p.part, parts, p.D,
+                             dweight ? dweight->data : nullptr, dbias ? dbias->data : nullptr, p.accumulate));
     }
     return TLC_OK;
 }

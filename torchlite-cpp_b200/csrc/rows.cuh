@@ -226,18 +226,31 @@ inline int sm_count() {
     return sms;
 }
 
+// A launch whose blocks may be set up while the kernel before it on the stream
+// still runs; the kernel begins with after_previous().
+template <class K, class... A>
+int launch_after(K kernel, unsigned grid, unsigned block, cudaStream_t s, const char* what, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    TLC_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+    count_launch();
+    return check_launch(what);
+}
+
 // ---- device helpers --------------------------------------------------------------------
 
-template <int VEC>
-struct FloatVec;
-template <>
-struct FloatVec<1> {
-    using T = float;
-};
-template <>
-struct FloatVec<4> {
-    using T = float4;
-};
+// Waits until the kernel before this one has ended and its writes are visible
+// (see launch_after; nothing of that kernel's may be touched before).
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the next kernel's blocks be set up from here on.
+__device__ __forceinline__ void next_may_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // VEC floats at p (16-byte aligned where VEC is 4).  load_once, store_once: streaming.
 template <int VEC>
