@@ -98,7 +98,7 @@ def reference(p, tokens):
 
 
 def check(got, want):
-    for i, (a, b) in enumerate(zip(got[0], want[0])):
+    for i, (a, b) in enumerate(zip(got[0], (w.detach() for w in want[0]))):
         if i == 3:
             assert torch.equal(a, b)
         else:
@@ -135,3 +135,85 @@ def test_training_step_in_a_graph():
     torch.cuda.synchronize()
     check(out, reference(p, other))
     check(again, reference(p, other))
+
+
+FIRST = """
+import sys
+sys.path.insert(0, {pkg!r})
+import torch, tlcuda
+x, w = torch.randn(40, 5001, device="cuda"), torch.randn(5001, device="cuda")
+t = torch.arange(40, device="cuda") % 7
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y, st = tlcuda.layer_norm(x, w, w)
+    back = tlcuda.layer_norm_backward(y, x, st, w)
+    e = tlcuda.embedding(x, t, 2.0)
+    d = tlcuda.embedding_backward(e, t, 7)
+    f = tlcuda.token_logprobs(x, t, top=5)
+    b = tlcuda.token_logprobs_backward(x, t, f[2], f[0], f[1], f[1])
+graph.replay()
+torch.cuda.synchronize()
+got = [y, st, *back, e, d, *f, b]
+y, st = tlcuda.layer_norm(x, w, w)
+f = tlcuda.token_logprobs(x, t, top=5)
+want = [y, st, *tlcuda.layer_norm_backward(y, x, st, w), tlcuda.embedding(x, t, 2.0),
+        tlcuda.embedding_backward(tlcuda.embedding(x, t, 2.0), t, 7), *f,
+        tlcuda.token_logprobs_backward(x, t, f[2], f[0], f[1], f[1])]
+assert all(torch.equal(a, c) for a, c in zip(got, want))
+print("captured first")
+"""
+
+
+def test_first_calls_of_a_process_captured():
+    """The set-up of a first call (kernel attributes, occupancy, the memory pool) inside a capture."""
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST.format(pkg=os.path.dirname(os.path.abspath(tlcuda.__file__)))],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
+
+
+def test_two_host_threads():
+    """Calls from two threads, each on its own stream, give each thread's own results."""
+    import threading
+    p, tokens = make()
+    inputs = [tokens, torch.roll(tokens, 2, 1).contiguous()]
+    want = [step(p, t) for t in inputs]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                got[i] = step(p, inputs[i])
+        s.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        for x, y in zip((*a[0], *a[1].values()), (*b[0], *b[1].values())):
+            assert torch.equal(x, y)
+
+
+def test_views_that_repeat_memory():
+    """Inputs of stride 0 (one row for all, one value for all) and the same token everywhere."""
+    row = torch.randn(300, device="cuda")
+    w = torch.randn(300, device="cuda")
+    x = row.expand(20, 300)
+    y, st = tlcuda.layer_norm(x, w)
+    assert torch.equal(y, tlcuda.layer_norm(x.contiguous(), w)[0])
+    one = torch.ones((), device="cuda").expand(300)
+    assert torch.equal(tlcuda.layer_norm(x, one, one)[0], tlcuda.layer_norm(x, one.contiguous(), one.contiguous())[0])
+    for a, b in zip(tlcuda.layer_norm_backward(x, x, st[:1].expand(20, 2), w),
+                    tlcuda.layer_norm_backward(x.contiguous(), x.contiguous(), st, w)):
+        assert torch.equal(a, b)
+    t = torch.full((), 7, device="cuda").expand(20)
+    assert torch.equal(tlcuda.embedding(x, t), x)
+    for a, b in zip(tlcuda.token_logprobs(x, t, top=3), tlcuda.token_logprobs(x.contiguous(), t.contiguous(), top=3)):
+        assert torch.equal(a, b)

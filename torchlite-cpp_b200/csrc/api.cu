@@ -63,6 +63,7 @@ int scratch_alloc(void** p, size_t bytes, cudaStream_t s) {
     // Keep freed pool memory instead of returning it to the driver, so
     // repeated calls do not pay for fresh allocations.
     TLC_TRY(device_once(once, [](int dev) -> int {
+        SetupDuringCapture relaxed;
         cudaMemPool_t pool;
         if (cudaDeviceGetDefaultMemPool(&pool, dev) == cudaSuccess) {
             uint64_t thr = ~0ull;

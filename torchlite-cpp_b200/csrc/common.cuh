@@ -66,10 +66,22 @@ int device_once(DeviceOnce& o, F&& setup, int* dev_out = nullptr) {
     return st;
 }
 
+// While one lives, the calling thread may make set-up calls that touch no
+// stream (attributes, occupancy, the memory pool) although it captures one:
+// a first call inside a capture works like any other.
+struct SetupDuringCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    SetupDuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~SetupDuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    SetupDuringCapture(const SetupDuringCapture&) = delete;
+    SetupDuringCapture& operator=(const SetupDuringCapture&) = delete;
+};
+
 // Raises a kernel's dynamic shared-memory limit on the current device.
 template <class K>
 int smem_limit_once(DeviceOnce& o, K kernel, int bytes) {
     return device_once(o, [&](int) -> int {
+        SetupDuringCapture relaxed;
         TLC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
         return TLC_OK;
     });

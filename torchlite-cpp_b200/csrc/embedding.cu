@@ -567,6 +567,7 @@ int max_clusters(int* out) {
     TLC_TRY(device_once(
         once,
         [](int d) -> int {
+            SetupDuringCapture relaxed;
             const int smem = (int)std::max(sizeof(SortSmem), sizeof(FillSmem));
             TLC_CUDA_TRY(cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             cudaLaunchConfig_t cfg{};
