@@ -427,32 +427,38 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(SumArgs p, int64_t units
     }
 }
 
-// The sum of `count` parts 0 from chunk `c` on, in their order.
-template <int VEC>
-__device__ __forceinline__ void add_parts(const SumArgs& p, int c, int count, int j, float (&a)[VEC]) {
-    constexpr int U = 8;
+// The sums of `count` parts 0 from chunk `c` on, in their order.
+template <int VEC, int VPT>
+__device__ __forceinline__ void add_parts(const SumArgs& p, int c, int count, int j, float (&a)[VPT][VEC]) {
+    constexpr int U = 4;
     for (int q = 0; q < count; q += U) {
-        float v[U][VEC];
+        float v[U][VPT][VEC];
 #pragma unroll
         for (int k = 0; k < U; ++k)
-            if (q + k < count) load_vec<VEC>(p.part + (int64_t)(c + q + k) * 2 * p.D + j, v[k]);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (q + k < count && j + i * 32 * VEC < p.D)
+                    load_vec<VEC>(p.part + (int64_t)(c + q + k) * 2 * p.D + j + i * 32 * VEC, v[k][i]);
 #pragma unroll
         for (int k = 0; k < U; ++k)
             if (q + k < count)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) a[e] += v[k][e];
+                for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) a[i][e] += v[k][i][e];
     }
 }
 
 // A run that crosses chunks: its first chunk's part 1, then part 0 of the
-// chunks behind it, in their order.  A warp takes a run and 32 * VEC columns;
-// runs of more than LONG chunks (one token in thousands of positions) are
-// shared by the block's warps, an eighth of the chunks each.
+// chunks behind it, in their order.  A warp takes a run and 32 * VEC * VPT
+// columns (a run is found by five loads one after the other, so a warp finds
+// few and sums much); runs of more than LONG chunks (one token in hundreds of
+// positions) are shared by the block's warps, an eighth of the chunks each.
 constexpr int LONG = 16;
-template <int VEC>
+template <int VEC, int VPT>
 __global__ void __launch_bounds__(256) embed_join_kernel(SumArgs p, int slices) {
     __shared__ int long_chunk[8], long_slice[8], long_count[8];
-    __shared__ float eighth[8][32 * VEC];
+    __shared__ __align__(16) float eighth[8][VPT][32 * VEC];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     after_previous();
     const int runs = *p.crossing;
@@ -461,10 +467,22 @@ __global__ void __launch_bounds__(256) embed_join_kernel(SumArgs p, int slices) 
     for (int64_t u0 = blockIdx.x; u0 < units; u0 += (int64_t)gridDim.x * 8) {
         const int64_t u = u0 + (int64_t)gridDim.x * warp;
         int count = 0;  // chunks behind the first
+        float a[VPT][VEC];
+        auto first_part = [&](int chunk, int j) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (j + i * 32 * VEC < p.D)
+                    load_vec<VEC>(p.part + ((int64_t)chunk * 2 + 1) * p.D + j + i * 32 * VEC, a[i]);
+        };
+        auto write = [&](uint32_t key, int j) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (j + i * 32 * VEC < p.D) write_row<VEC>(p, key, j + i * 32 * VEC, a[i]);
+        };
         if (u < units) {
             // neighbouring warps take different runs: the slices of a long one go to different blocks
             const int slice = (int)(u / runs), chunk = p.crossing[1 + (int)(u - (int64_t)slice * runs)];
-            const int j = slice * (32 * VEC) + lane * VEC;
+            const int j = slice * (32 * VEC * VPT) + lane * VEC;
             const uint32_t key = p.list[(int64_t)(chunk + 1) * p.ch - 1].x;
             for (;;) {  // does the run reach into chunk + 1 + count + lane?
                 const int64_t begin = (int64_t)(chunk + 1 + count + lane) * p.ch;
@@ -473,11 +491,10 @@ __global__ void __launch_bounds__(256) embed_join_kernel(SumArgs p, int slices) 
                 count += full;
                 if (full < 32) break;
             }
-            if (count <= LONG && j < p.D) {
-                float a[VEC];
-                load_vec<VEC>(p.part + ((int64_t)chunk * 2 + 1) * p.D + j, a);
-                add_parts<VEC>(p, chunk + 1, count, j, a);
-                write_row<VEC>(p, key, j, a);
+            if (count <= LONG) {
+                first_part(chunk, j);
+                add_parts<VEC, VPT>(p, chunk + 1, count, j, a);
+                write(key, j);
             }
             if (lane == 0) long_chunk[warp] = chunk, long_slice[warp] = slice;
         }
@@ -486,26 +503,28 @@ __global__ void __launch_bounds__(256) embed_join_kernel(SumArgs p, int slices) 
         for (int q = 0; q < 8; ++q) {
             const int n = long_count[q];
             if (n == 0) continue;
-            const int chunk = long_chunk[q], j = long_slice[q] * (32 * VEC) + lane * VEC;
+            const int chunk = long_chunk[q], j = long_slice[q] * (32 * VEC * VPT) + lane * VEC;
             const int per = (n + 7) / 8, c0 = min(n, warp * per), c1 = min(n, c0 + per);
-            float a[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) a[e] = 0.0f;
-            if (j < p.D) {
-                if (warp == 0) load_vec<VEC>(p.part + ((int64_t)chunk * 2 + 1) * p.D + j, a);
-                add_parts<VEC>(p, chunk + 1 + c0, c1 - c0, j, a);
-            }
-            store_vec<VEC>(&eighth[warp][lane * VEC], a);
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) a[i][e] = 0.0f;
+            if (warp == 0) first_part(chunk, j);
+            add_parts<VEC, VPT>(p, chunk + 1 + c0, c1 - c0, j, a);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) store_vec<VEC>(&eighth[warp][i][lane * VEC], a[i]);
             __syncthreads();
-            if (warp == 0 && j < p.D) {
+            if (warp == 0) {
 #pragma unroll
-                for (int w = 1; w < 8; ++w) {
-                    float v[VEC];
-                    load_vec<VEC>(&eighth[w][lane * VEC], v);
+                for (int w = 1; w < 8; ++w)
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) a[e] += v[e];
-                }
-                write_row<VEC>(p, p.list[(int64_t)(chunk + 1) * p.ch - 1].x, j, a);
+                    for (int i = 0; i < VPT; ++i) {
+                        float v[VEC];
+                        load_vec<VEC>(&eighth[w][i][lane * VEC], v);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) a[i][e] += v[e];
+                    }
+                write(p.list[(int64_t)(chunk + 1) * p.ch - 1].x, j);
             }
             __syncthreads();
         }
@@ -554,9 +573,10 @@ int launch_sums(const SumArgs& p, cudaStream_t s) {
     TLC_TRY(launch_after(embed_sum_kernel<VEC, VPT>, (unsigned)blocks, 256, s, kBwd, p, chunks * slices, slices));
     if (chunks == 1) return TLC_OK;  // no run crosses
     // the number of crossing runs is on the device: enough blocks to keep every SM busy
-    const int thin = (p.D + 32 * VEC - 1) / (32 * VEC);
-    const unsigned grid = (unsigned)std::min<int64_t>((chunks * thin + 7) / 8, (int64_t)sm_count() * 4);
-    return launch_after(embed_join_kernel<VEC>, grid, 256, s, kBwd, p, thin);
+    constexpr int WIDE = 2;
+    const int wide = (p.D + 32 * VEC * WIDE - 1) / (32 * VEC * WIDE);
+    const unsigned grid = (unsigned)std::min<int64_t>((chunks * wide + 7) / 8, (int64_t)sm_count() * 4);
+    return launch_after(embed_join_kernel<VEC, WIDE>, grid, 256, s, kBwd, p, wide);
 }
 
 // The most clusters of the sort kernel that run at once on the current device.
