@@ -8,7 +8,10 @@
 // Bound by HBM: the forward moves 8 bytes an element (x in, y out), the
 // backward 12 (x and g in, dx out).  So a row is read once, into registers,
 // and both statistics come from there (the mean first, then the squares of
-// the differences: no cancellation).
+// the differences: no cancellation).  Measured (GPU time): forward 8192 x 768
+// 10.6 us (4.8 TB/s), 4096 x 16384 87 us (6.2 TB/s), unaligned 4099 x 5001
+// 34.8 us (4.7 TB/s); backward 8192 x 768 19.6 us (3.9 TB/s), 8192 x 8192
+// 144 us (5.6 TB/s), unaligned 16000 x 1001 43 us (4.5 TB/s).
 #include <algorithm>
 #include <cmath>
 
@@ -99,8 +102,8 @@ __global__ void __launch_bounds__(THREADS <= 32 ? 128 : THREADS, THREADS <= 32 ?
     }
 }
 
-// Rows too long for the registers of a block: the row is read three times
-// (from L2 after the first).
+// Rows too long for the registers of a block (above 32768 columns, 16384
+// unaligned): the row is read three times (from L2 after the first).
 __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(LnFwd p) {
     __shared__ float red[2][32];
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(BT, 1) ln_bwd_kernel(LnBwd p) {
     }
 }
 
-// Rows too long for that: dx alone, the row read twice ...
+// Rows too long for that (above 16384 columns): dx alone, the row read twice ...
 __global__ void __launch_bounds__(1024) ln_bwd_long_kernel(LnBwd p) {
     __shared__ float red[2][64];
     const float inv = 1.0f / (float)p.D;
@@ -461,7 +464,8 @@ int launch_fwd(const LnFwd& p, cudaStream_t s) {
 }
 
 // 16 to 32 values a thread: many small blocks keep more rows in flight than few large ones
-// (and than rings of copies ahead: 8192 x 768 11 us, 14 through a ring).
+// (4099 x 5001: 35 us by 256 threads, 46 by 512, 75 by 1024) and than rings of copies ahead
+// (8192 x 768: 10.6 us, 14 through a ring).
 template <int VEC>
 int pick_fwd(const LnFwd& p, cudaStream_t s) {
     const int n = (p.D + VEC - 1) / VEC;  // vectors a row

@@ -60,25 +60,34 @@ struct TokenRef {
         const int64_t o = map.offset(i);
         return wide ? static_cast<const int64_t*>(data)[o] : static_cast<int64_t>(static_cast<const int32_t*>(data)[o]);
     }
-    // The tokens first + k * step below end (-1 behind it).  All loads are issued before the first
-    // is waited for, which a loop over get() with its branches does not get from the compiler.
+    // N tokens, those with in[k] (-1 for the others).  All loads are issued before the first is
+    // waited for, which a loop over get() with its branches does not get from the compiler.
     template <int N>
-    __device__ __forceinline__ void get(int64_t first, int64_t step, int64_t end, int64_t (&t)[N]) const {
+    __device__ __forceinline__ void get(const int64_t (&i)[N], const bool (&in)[N], int64_t (&t)[N]) const {
         int64_t o[N];
         if (map.nd <= 1) {
 #pragma unroll
-            for (int k = 0; k < N; ++k) o[k] = (first + k * step) * map.st[0];
+            for (int k = 0; k < N; ++k) o[k] = i[k] * map.st[0];
         } else {
 #pragma unroll
-            for (int k = 0; k < N; ++k) o[k] = first + k * step < end ? map.offset(first + k * step) : 0;
+            for (int k = 0; k < N; ++k) o[k] = in[k] ? map.offset(i[k]) : 0;
         }
         if (wide) {
 #pragma unroll
-            for (int k = 0; k < N; ++k) t[k] = first + k * step < end ? static_cast<const int64_t*>(data)[o[k]] : -1;
+            for (int k = 0; k < N; ++k) t[k] = in[k] ? static_cast<const int64_t*>(data)[o[k]] : -1;
         } else {
 #pragma unroll
-            for (int k = 0; k < N; ++k) t[k] = first + k * step < end ? static_cast<const int32_t*>(data)[o[k]] : -1;
+            for (int k = 0; k < N; ++k) t[k] = in[k] ? static_cast<const int32_t*>(data)[o[k]] : -1;
         }
+    }
+    // The tokens first + k * step below end.
+    template <int N>
+    __device__ __forceinline__ void get(int64_t first, int64_t step, int64_t end, int64_t (&t)[N]) const {
+        int64_t i[N];
+        bool in[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) i[k] = first + k * step, in[k] = i[k] < end;
+        get(i, in, t);
     }
 };
 
