@@ -86,12 +86,14 @@ struct Run {
     }
 };
 
-// Adds values to a run, two at a time: 8 instructions for two values.
+// Adds values to a run, two at a time: 8 instructions for two values.  The lanes
+// of a warp add together and share the running maximum, so that it moves a few
+// times a row (each lane's own moves in some lane in nearly every batch).
 struct PairRun {
-    float m = -INFINITY;
-    // batch `where` has m, batch `where2` the second largest of the batches' maxima, `rest` is the
-    // largest of the others' (all three NaN from the first NaN on)
-    float second = -INFINITY, rest = -INFINITY;
+    float m = -INFINITY;  // the warp's
+    // for the alternatives, of this lane alone: batch `where` has the largest value `most`, batch
+    // `where2` the second largest of the batches' maxima, `rest` is the largest of the others'
+    float most = -INFINITY, second = -INFINITY, rest = -INFINITY;
     int where = 0, where2 = 0;
     Pair l, w, a2;
     float a;
@@ -105,22 +107,24 @@ struct PairRun {
             top = max3_nan(top, v[i], other);
             low = min3(low, v[i], other);
         }
-        if (!(top <= m)) {  // also when top is NaN
-            const float to = max_nan(top, m);
+        if (__any_sync(0xffffffffu, !(top <= m))) {  // also when top is NaN
+            float to = max_nan(top, m);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) to = max_nan(to, __shfl_xor_sync(0xffffffffu, to, o));
             if (m != -INFINITY) {
                 const float y = max_nan((m - to) * a, kFloor), c = ex2(y);
                 w = mul2(pair(c, c), fma2(pair(y, y), l, w));
                 l = mul2(pair(c, c), l);
             }
-            rest = max_nan(rest, second);
-            second = m, where2 = where;
-            m = to, where = batch;
-        } else if (top > second) {
-            rest = max_nan(rest, second);
-            second = top, where2 = batch;
-        } else {
-            rest = max_nan(rest, top);
+            m = to;
         }
+        // a new largest value pushes the old one to second place, a new second the old second out
+        const bool first = top > most, one_of_two = top > second;
+        rest = fmaxf(rest, one_of_two ? second : top);
+        second = fmaxf(second, fminf(top, most));
+        where2 = first ? where : one_of_two ? batch : where2;
+        most = fmaxf(most, top);
+        where = first ? batch : where;
         const float base = m == -INFINITY ? 0.0f : -m;
         const Pair shift = pair(base, base);
         // masked values need the bound on their exponent; without any it is left out
@@ -167,6 +171,14 @@ __device__ __forceinline__ Run warp_run(Run r, float a) {
     float s[2] = {r.l, r.w};
     warp_sum(s);
     r.m = to, r.l = s[0], r.w = s[1];
+    return r;
+}
+// The same where the lanes have one maximum already.
+__device__ __forceinline__ Run warp_run(const PairRun& own) {
+    Run r = own.sum();
+    float s[2] = {r.l, r.w};
+    warp_sum(s);
+    r.l = s[0], r.w = s[1];
     return r;
 }
 
@@ -373,7 +385,7 @@ struct Feed {
             ++batch;
             rest -= STEP;
         } while (rest > 0);
-        if (alone_at >= 0) {
+        if (__any_sync(0xffffffffu, alone_at >= 0)) {
             const float v[1] = {alone};
             own.add(v, -1);
         }
@@ -443,7 +455,7 @@ __global__ void __launch_bounds__(256, 3) lp_warp_kernel(LpFwd p) {
         const Asked asked = lane == 0 ? Asked(p, r, x) : Asked();
         PairRun own(p.a);
         feed.add_row(part, own);
-        const Run s = warp_run(own.sum(), p.a);
+        const Run s = warp_run(own);
         if (lane == 0) row_results(p, r, asked, s);
         if constexpr (TOP) {
             uint64_t* cand = cands[warp];
@@ -452,7 +464,7 @@ __global__ void __launch_bounds__(256, 3) lp_warp_kernel(LpFwd p) {
             if (s.m == s.m) {
                 // Each lane has three maxima of disjoint sets of its values.  What `top` of
                 // these 96 reach, `top` values reach.
-                const uint32_t most = order_of(own.m), second = order_of(own.second), rest = order_of(own.rest);
+                const uint32_t most = order_of(own.most), second = order_of(own.second), rest = order_of(own.rest);
                 const uint32_t bound = highest_bound(p.top, most, second, rest);
                 if (lane == 0) founds[warp] = 0;
                 __syncwarp();
@@ -523,8 +535,9 @@ struct LpSmem {
 };
 
 // The part's `k` largest keys in order, into sm.best (k <= part.n values; the
-// rest of sm.best is 0).  top: the largest value of this thread (-inf: none),
+// rest of sm.best is 0).  top: the largest number of this thread (-inf: none),
 // which its batch `where` has (-1: its single value), rest: that of the others.
+// sm.row_m, written by warp 0 before, is NaN if the part has one.
 template <int T>
 __device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top, float rest, int where) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -563,9 +576,9 @@ __device__ void part_top(LpSmem<T>& sm, const Part& part, int k, float top, floa
     }
     __syncthreads();
     int found = sm.found;
-    if (found > CAP) {
-        // Too many values reach the bound (equal logits, or few that are not
-        // masked): find the k-th largest key digit by digit, reading the part
+    if (found > CAP || sm.row_m != sm.row_m) {
+        // NaN, or too many values that reach the bound (equal logits, or few
+        // that are not masked): find the k-th largest key digit by digit, reading the part
         // once for each of the 8 digits, then take the k keys from it up.
         uint64_t prefix = 0;
         if (tid == 0) sm.need = k;
@@ -635,7 +648,7 @@ __global__ void __launch_bounds__(T) lp_row_kernel(LpFwd p, int C) {
         const Asked asked = tid == 0 && rank == 0 ? Asked(p, r, x) : Asked();
         PairRun own(p.a);
         feed.add_row(part, own);
-        const Run s = warp_run(own.sum(), p.a);
+        const Run s = warp_run(own);
         if (lane == 0) sm.m[warp] = s.m, sm.l[warp] = s.l, sm.w[warp] = s.w;
         __syncthreads();
         if (warp == 0) {
@@ -646,7 +659,7 @@ __global__ void __launch_bounds__(T) lp_row_kernel(LpFwd p, int C) {
         }
         const int k = min(p.top, part.n);
         if (k > 0)
-            part_top(sm, part, k, own.m, max_nan(own.second, own.rest), own.where);
+            part_top(sm, part, k, own.most, fmaxf(own.second, own.rest), own.where);
         else if (p.top > 0 && tid < kMaxTop)
             sm.best[tid] = 0;
         __syncthreads();
