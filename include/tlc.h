@@ -353,7 +353,10 @@ int tlc_embedding(const tlc_tensor* weight, const tlc_index* tokens, float scale
  * zeros for tokens that do not occur; with accumulate != 0 these sums are
  * added to what dweight holds (rows that do not occur stay as they are).
  * Tokens outside [0, V), -1 among them, take no part.  The positions are
- * sorted by token, so each row's additions have one fixed order. */
+ * sorted by token, so each row's additions have one fixed order.  Takes
+ * scratch of an eighth of grad's size at most (two rows at least) and 20 bytes a position from the
+ * device's memory pool; at most 2^31 - 8193 positions and 2^31 - 2 rows
+ * (TLC_ERR_UNSUPPORTED). */
 int tlc_embedding_backward(const tlc_tensor* grad, const tlc_index* tokens, float scale,
                            tlc_tensor* dweight, int accumulate, void* stream);
 

@@ -173,6 +173,20 @@ def test_beyond_32_bits():
 
 
 @pytest.mark.gpu
+def test_a_table_of_many_rows():
+    """More rows than the marks of all blocks hold at once (65536 a block), and three digits a token."""
+    rows, d = 9_700_000, 3
+    t = torch.tensor([0, rows - 1, 4_000_000, rows - 1, 7_340_031, 7_340_032, -1, 8_000_001, rows], device="cuda")
+    g = torch.arange(1, 28, device="cuda", dtype=torch.float32).view(9, 3)
+    got = tlcuda.embedding_backward(g, t, dweight=torch.full((rows, d), 5.0, device="cuda"))
+    want = torch.zeros(rows, d, device="cuda")
+    for i, v in enumerate(t.tolist()):
+        if 0 <= v < rows:
+            want[v] += g[i]  # whole numbers: exact
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_same_bits_streams_and_graphs():
     rng = np.random.default_rng(4)
     t = dev(np.minimum(np.exp(rng.random(9000) * np.log(2000)).astype(np.int64), 1999))

@@ -66,7 +66,10 @@ def host(t):
 SHAPES = [(1, 1), (3, 1), (5, 2), (1, 3), (2, 3, 31), (7, 32), (9, 33), (4, 128), (5, 129), (17, 257), (3, 512),
           (3, 513), (40, 768), (2, 1001), (6, 1024), (3, 1025), (5, 1028), (2, 2048), (3, 2052), (2, 4097),
           (3, 5001), (2, 8192), (2, 8196), (2, 8191), (3, 16384), (2, 16385), (2, 40000), (1500, 24), (700, 768),
-          (2000, 8), (333, 2049), (64, 16400)]
+          (2000, 8), (333, 2049), (64, 16400),
+          # the ends of the backward's ranges of columns a thread, and of the forward's
+          (5, 769), (4, 1536), (4, 1537), (3, 4096), (3, 6148), (2, 10001), (3, 12288), (2, 12289), (2, 16380), (2, 32768),
+          (2, 32772), (1200, 130), (700, 260), (400, 515), (310, 1540)]
 
 
 @pytest.mark.gpu
