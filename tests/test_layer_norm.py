@@ -263,6 +263,48 @@ def test_streams_and_graphs():
         assert all(torch.equal(p, q) for p, q in zip(o, (y0, s0, *b0)))
 
 
+def around_the_mean(x, w, b, eps):
+    """What `reference` gives, with the bounds of a mean that the differences to a first one correct.
+
+    The first mean is off by at most SUM roundings of mean |x|, which is `first`; the sum of the
+    differences to it loses SUM roundings of their mean, at most mean |x - mean| + first."""
+    x = x.astype(np.float64)
+    w, bb = w.astype(np.float64), b.astype(np.float64)
+    mean = x.mean(-1, keepdims=True)
+    var = ((x - mean) ** 2).mean(-1, keepdims=True)
+    rstd = 1 / np.sqrt(var + eps)
+    y = (x - mean) * rstd * w + bb
+    first = SUM * U * np.abs(x).mean(-1, keepdims=True)
+    d_mean = (SUM + 4) * U * (np.abs(x - mean).mean(-1, keepdims=True) + first)
+    # the squares of the differences, whose mean is at most 2 (var + first^2), lose SUM + 6 roundings
+    rel = 0.5 * (SUM + 6) * U * 2 * (var + first ** 2) / (var + eps) + 3 * U
+    tol = rstd * np.abs(w) * (d_mean + (np.abs(x - mean) + first) * 4 * U + np.abs(x - mean) * rel) + 2 * U * (
+        np.abs(y) + np.abs(bb))
+    return y, mean, rstd, tol, U * np.abs(mean) + d_mean, rel
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [5, 100, 768, 1030, 5001, 8192, 12001, 40000])
+@pytest.mark.parametrize("off", [0, 3], ids=["aligned", "off 16 bytes"])
+def test_rows_far_from_zero(d, off):
+    """Rows of one value, whose partial sums round, and rows whose mean is 1e3 to 1e5 times their spread."""
+    rng = np.random.default_rng(d)
+    spread = rng.standard_normal((4, d))
+    rows = [np.full(d, v) for v in (0.1, 1000.1, -98765.43, 1e-3)]
+    rows += [v + spread[i] * s for i, (v, s) in enumerate([(1e3, 1.0), (-1e4, 1.0), (1e5, 1.0), (98765.43, 0.01)])]
+    x = np.stack(rows).astype(np.float32)
+    w = (1 + 0.3 * rng.standard_normal(d)).astype(np.float32)
+    b = rng.standard_normal(d).astype(np.float32)
+    buf = torch.empty(x.size + off, device="cuda")
+    vx = buf[off:].view(x.shape)
+    vx.copy_(dev(x))
+    y, stats = tlcuda.layer_norm(vx, dev(w), dev(b), 1e-5)
+    ref, mean, rstd, tol, d_mean, rel = around_the_mean(x, w, b, 1e-5)
+    assert (np.abs(host(y) - ref) <= tol).all()
+    st = host(stats).astype(np.float64)
+    assert (np.abs(st[..., :1] - mean) <= d_mean).all() and (np.abs(st[..., 1:] / rstd - 1) <= rel).all()
+
+
 F = "tlc_layer_norm"
 B = "tlc_layer_norm_backward"
 A, Z = 1 << 20, 1 << 30  # addresses far apart

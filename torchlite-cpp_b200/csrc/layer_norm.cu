@@ -7,11 +7,15 @@
 //
 // Bound by HBM: the forward moves 8 bytes an element (x in, y out), the
 // backward 12 (x and g in, dx out).  So a row is read once, into registers,
-// and both statistics come from there (the mean first, then the squares of
-// the differences: no cancellation).  Measured (GPU time): forward 8192 x 768
-// 10.6 us (4.8 TB/s), 4096 x 16384 87 us (6.2 TB/s), unaligned 4099 x 5001
-// 34.8 us (4.7 TB/s); backward 8192 x 768 19.6 us (3.9 TB/s), 8192 x 8192
-// 144 us (5.6 TB/s), unaligned 16000 x 1001 43 us (4.5 TB/s).
+// and both statistics come from there: a first mean, then the sums of the
+// differences to it and of their squares.  A sum of D values is off by some
+// roundings of its size, which a row whose mean is many times its spread would
+// feel in every result (of a row of 1000.1 alone xhat was 0.06), so the
+// differences' own mean is taken off them and off the variance.
+// Measured (GPU time): forward 8192 x 768 10.4 us (4.8 TB/s), 4096 x 16384
+// 88 us (6.1 TB/s), unaligned 4099 x 5001 34.8 us (4.7 TB/s); backward 8192 x
+// 768 19.8 us (3.8 TB/s), 8192 x 8192 144 us (5.6 TB/s), unaligned 16000 x 1001
+// 43 us (4.5 TB/s).
 #include <algorithm>
 #include <cmath>
 
@@ -19,6 +23,18 @@
 
 namespace tlc {
 namespace {
+
+// What a first mean lacks, and 1 / sqrt(var + eps), from the sums of the differences to it and of
+// their squares; xhat of a difference d is d * rstd + shift.
+struct Spread {
+    float off, rstd, shift;
+    __device__ __forceinline__ Spread(const float (&s)[2], int D, float eps) {
+        off = __fdiv_rn(s[0], (float)D);
+        const float var = fmaf(-off, off, __fdiv_rn(s[1], (float)D));
+        rstd = __frsqrt_rn((var < 0.0f ? 0.0f : var) + eps);  // a NaN stays one
+        shift = -off * rstd;
+    }
+};
 
 struct LnFwd {
     const float *x, *w, *b;
@@ -36,7 +52,8 @@ template <int VEC, int VPT, int THREADS>
 __global__ void __launch_bounds__(THREADS <= 32 ? 128 : THREADS, THREADS <= 32 ? 1 : 1024 / THREADS)
     ln_fwd_kernel(LnFwd p) {
     constexpr int RPB = THREADS <= 32 ? 128 / THREADS : 1;
-    __shared__ float red[2][32];
+    constexpr bool FEW = VEC * VPT < 32;  // 32 values spill with it (4096 x 16384: 90.6 us for 87.8)
+    __shared__ float red[32], red2[64];
     const int t = threadIdx.x % THREADS, sub = threadIdx.x / THREADS;
     const int n = p.D / VEC;
     const int whole = n / THREADS + (t < n % THREADS ? 1 : 0);  // this thread's vectors of a row
@@ -55,19 +72,24 @@ __global__ void __launch_bounds__(THREADS <= 32 ? 128 : THREADS, THREADS <= 32 ?
             if (i < mine)
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) s[0] += v[i][k];
-        group_sum<THREADS>(s, red[0]);
-        const float mean = __fdiv_rn(s[0], (float)p.D);  // exact for rows of one value
-        float q[1] = {0.0f};
+        group_sum<THREADS, FEW>(s, red);
+        const float mean = __fdiv_rn(s[0], (float)p.D);
+        float d[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
             if (i < mine)
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
                     v[i][k] -= mean;
-                    q[0] = fmaf(v[i][k], v[i][k], q[0]);
+                    d[0] += v[i][k];
+                    d[1] = fmaf(v[i][k], v[i][k], d[1]);
                 }
-        group_sum<THREADS>(q, red[1]);
-        const float rstd = __frsqrt_rn(__fdiv_rn(q[0], (float)p.D) + p.eps);
+        group_sum<THREADS, FEW>(d, red2);
+        const Spread sp(d, p.D, p.eps);
+        if (p.stats && t == 0 && live) {
+            p.stats[2 * r] = mean + sp.off;
+            p.stats[2 * r + 1] = sp.rstd;
+        }
         float* yr = p.out + r * p.D + t * VEC;
         const float* w = p.w + t * VEC;
         const float* b = p.b + t * VEC;
@@ -79,7 +101,7 @@ __global__ void __launch_bounds__(THREADS <= 32 ? 128 : THREADS, THREADS <= 32 ?
                     load_vec<VEC>(w + i * THREADS * VEC, wv);
                     load_vec<VEC>(b + i * THREADS * VEC, bv);
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) v[i][k] = fmaf(v[i][k] * rstd, wv[k], bv[k]);
+                    for (int k = 0; k < VEC; ++k) v[i][k] = fmaf(fmaf(v[i][k], sp.rstd, sp.shift), wv[k], bv[k]);
                     store_once<VEC>(yr + i * THREADS * VEC, v[i]);
                 }
         } else {
@@ -88,16 +110,12 @@ __global__ void __launch_bounds__(THREADS <= 32 ? 128 : THREADS, THREADS <= 32 ?
                 if (i < mine) {
 #pragma unroll
                     for (int k = 0; k < VEC; ++k) {
-                        v[i][k] *= rstd;
+                        v[i][k] = fmaf(v[i][k], sp.rstd, sp.shift);
                         if (p.w) v[i][k] *= w[i * THREADS * VEC + k];
                         if (p.b) v[i][k] += b[i * THREADS * VEC + k];
                     }
                     store_once<VEC>(yr + i * THREADS * VEC, v[i]);
                 }
-        }
-        if (p.stats && t == 0 && live) {
-            p.stats[2 * r] = mean;
-            p.stats[2 * r + 1] = rstd;
         }
     }
 }
@@ -105,30 +123,31 @@ __global__ void __launch_bounds__(THREADS <= 32 ? 128 : THREADS, THREADS <= 32 ?
 // Rows too long for the registers of a block (above 32768 columns, 16384
 // unaligned): the row is read three times (from L2 after the first).
 __global__ void __launch_bounds__(1024) ln_fwd_long_kernel(LnFwd p) {
-    __shared__ float red[2][32];
+    __shared__ float red[32], red2[64];
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const float* xr = p.x + p.xm.offset(r);
         float s[1] = {0.0f};
         for (int64_t j = threadIdx.x; j < p.D; j += 1024) s[0] += xr[j];
-        group_sum<1024>(s, red[0]);
-        const float mean = __fdiv_rn(s[0], (float)p.D);  // exact for rows of one value
-        float q[1] = {0.0f};
+        group_sum<1024>(s, red);
+        const float mean = __fdiv_rn(s[0], (float)p.D);
+        float d[2] = {0.0f, 0.0f};
         for (int64_t j = threadIdx.x; j < p.D; j += 1024) {
-            const float d = xr[j] - mean;
-            q[0] = fmaf(d, d, q[0]);
+            const float v = xr[j] - mean;
+            d[0] += v;
+            d[1] = fmaf(v, v, d[1]);
         }
-        group_sum<1024>(q, red[1]);
-        const float rstd = __frsqrt_rn(__fdiv_rn(q[0], (float)p.D) + p.eps);
+        group_sum<1024>(d, red2);
+        const Spread sp(d, p.D, p.eps);
         float* yr = p.out + r * p.D;
         for (int64_t j = threadIdx.x; j < p.D; j += 1024) {
-            float y = (xr[j] - mean) * rstd;
+            float y = fmaf(xr[j] - mean, sp.rstd, sp.shift);
             if (p.w) y *= p.w[j];
             if (p.b) y += p.b[j];
             yr[j] = y;
         }
         if (p.stats && threadIdx.x == 0) {
-            p.stats[2 * r] = mean;
-            p.stats[2 * r + 1] = rstd;
+            p.stats[2 * r] = mean + sp.off;
+            p.stats[2 * r + 1] = sp.rstd;
         }
     }
 }

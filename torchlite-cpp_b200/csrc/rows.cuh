@@ -333,8 +333,9 @@ __device__ __forceinline__ void warp_sum(float (&v)[N]) {
 
 // Sums of N values over THREADS threads (at most 32: neighbouring lanes; else
 // the whole block), in every thread.  `red` holds THREADS / 32 * N floats that
-// nobody else uses until all threads have passed one more block barrier.
-template <int THREADS, int N>
+// nobody else uses until all threads have passed one more block barrier.  FEW:
+// only as many lanes as there are warps meet at the end: fewer shuffles, some registers.
+template <int THREADS, bool FEW = false, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* red) {
     if constexpr (THREADS <= 32) {
         warp_sum<THREADS>(v);
@@ -346,8 +347,9 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* red) {
             for (int n = 0; n < N; ++n) red[warp * N + n] = v[n];
         __syncthreads();
 #pragma unroll
-        for (int n = 0; n < N; ++n) v[n] = lane < THREADS / 32 ? red[lane * N + n] : 0.0f;
-        warp_sum(v);
+        for (int n = 0; n < N; ++n)
+            v[n] = FEW ? red[lane % (THREADS / 32) * N + n] : lane < THREADS / 32 ? red[lane * N + n] : 0.0f;
+        warp_sum<FEW ? THREADS / 32 : 32>(v);
     }
 }
 
