@@ -447,9 +447,10 @@ __global__ void __launch_bounds__(256) ln_bwd_cols_kernel(LnBwd p, int64_t rows_
 }
 
 // dw = sum of the blocks' sums in their order: 32 columns a block, 16 warps
-// over the parts.  Columns [0, D) are dw's, [D, 2D) db's.
-__global__ void __launch_bounds__(512) ln_bwd_finish_kernel(const float* __restrict__ part, int parts, int D,
-                                                            float* dw, float* db, int accumulate) {
+// over the parts.  Columns [0, D) are dw's, [D, 2D) db's.  `part` is still being
+// written when this kernel's blocks are set up: not __restrict__.
+__global__ void __launch_bounds__(512)
+    ln_bwd_finish_kernel(const float* part, int parts, int D, float* dw, float* db, int accumulate) {
     __shared__ float red[16][33];
     after_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
