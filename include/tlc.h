@@ -369,7 +369,7 @@ int tlc_embedding_backward(const tlc_tensor* grad, const tlc_index* tokens, floa
  *     order, equal logits by the lower token, with their log p.
  * Each output may be NULL (tokens too without logprobs; the two top_ ones
  * exactly when top is 0).  0 <= top <= min(V, 32), above 32
- * TLC_ERR_UNSUPPORTED; scale must be finite and > 0.
+ * TLC_ERR_UNSUPPORTED; scale must be > 0 and at most 2^100.
  * Token -1: none is asked for, logprobs 0 (the row's other results as usual);
  * any other token outside [0, V): NaN.  A row of -inf alone has no
  * distribution: log-probabilities -inf, entropy 0.  A NaN or +inf in a row

@@ -397,6 +397,26 @@ def test_refusals():
     assert refused("tlc_token_logprobs", x, t, 1.0, lp, H, st, 33, tl, tt)[1] == 2
 
 
+@pytest.mark.parametrize("scale", [2.0 ** 100 * (1 + 2.0 ** -23), 1e31, 2.0 ** 127, 2.4e38, 3.4e38, 1e-46, -0.0])
+def test_scales_out_of_range(scale):
+    """Above 2^100 scale * log2 e, or scale times a gradient, would leave float32; 1e-46 is 0 in it."""
+    x, t, lp, st, H = view((4, 50)), index((4,), data=Z), view((4,), data=2 * Z), view((4, 2), data=3 * Z), view((4,), data=4 * Z)
+    text, status = refused("tlc_token_logprobs", x, t, scale, lp, H, st, 0, None, None)
+    assert status == 1 and "scale" in text
+    text, status = refused("tlc_token_logprobs_backward", x, t, st, H, lp, H, scale, view((4, 50), data=6 * Z))
+    assert status == 1 and "scale" in text
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [40, 2000, 30001])
+@pytest.mark.parametrize("scale", [2.0 ** 100, 1e20, 2.0 ** -100])
+def test_scales_at_the_ends_of_the_range(V, scale):
+    """A huge scale leaves the largest logit and its equals (differences are 1/2 at least), a tiny one all alike."""
+    x = np.round(logits((5, V), V) * 2) / 2
+    x[3, V // 2] = NINF
+    check(x, np.array([int(np.argmax(x[0])), 0, V - 1, V // 2, -1]), scale, 5)
+
+
 def test_refusals_backward():
     x, t, st, H = view((4, 50)), index((4,), data=Z), view((4, 2), data=2 * Z), view((4,), data=3 * Z)
     g, h, d = view((4,), data=4 * Z), view((4,), data=5 * Z), view((4, 50), data=6 * Z)

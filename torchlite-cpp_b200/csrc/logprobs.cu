@@ -883,9 +883,11 @@ int launch_row(const LpFwd& p, cudaStream_t s) {
     return check_launch(kFwd);
 }
 
+// Above 2^127 scale * log2 e is infinite and the row's maximum gave 0 * inf; the gradient's
+// constants, scale times the gradients times up to 1000, leave float32 before that.
 int check_scale(float scale, const char* op) {
-    if (std::isfinite(scale) && scale > 0.0f) return TLC_OK;
-    return set_error(TLC_ERR_INVALID_ARGUMENT, std::string(op) + ": scale must be positive and finite");
+    if (scale > 0.0f && scale <= 0x1p100f) return TLC_OK;
+    return set_error(TLC_ERR_INVALID_ARGUMENT, std::string(op) + ": scale must be positive and at most 2^100");
 }
 
 // tokens (and others) have the shape of the logits without their last dim
