@@ -319,7 +319,8 @@ int tlc_flash_attention_backward(const tlc_tensor* grad_out, const tlc_tensor* q
  * Layer norm, embedding lookup and token log-probabilities with their
  * gradients, fp32 (the reference has nn::LayerNorm, nn::Embedding and
  * cross-entropy on the CPU, nn.h:56-630 and loss.cpp:12-103; these follow the
- * formulas, not its order of additions: sums are trees in fp32).
+ * formulas, not its order of additions: a sum in fp32 is one of many short
+ * running sums, whose lengths stand with each call).
  * Inputs are any views with strides >= 0 (a view whose last dim has stride 1 is
  * read in place, any other is copied first); outputs are contiguous, are
  * overwritten unless said otherwise, and may not lie over inputs or each other
@@ -338,7 +339,12 @@ int tlc_layer_norm(const tlc_tensor* x, const tlc_tensor* weight, const tlc_tens
  *   dx = rstd (gw - mean(gw) - xhat mean(gw xhat)),
  *   dweight = sum over rows of grad xhat,  dbias = sum over rows of grad.
  * NULL skips one.  accumulate != 0 adds to what the outputs hold (as
- * tlc_matmul_backward does; for dx, a residual branch's gradient). */
+ * tlc_matmul_backward does; for dx, a residual branch's gradient).  A sum over a
+ * row: every 1024th value of a long row in a thread (at most 32 up to 16384
+ * columns), then a tree.  dweight and dbias: a running sum over the rows that a
+ * group of threads takes, one in (SMs * 512 / threads a row), so rows / 148 above
+ * 4096 columns and rows / 9472 up to 128; above 16384 columns at most 128 rows
+ * (more beyond 8388480 rows); then these sums in a fixed order. */
 int tlc_layer_norm_backward(const tlc_tensor* grad, const tlc_tensor* x, const tlc_tensor* stats,
                             const tlc_tensor* weight, tlc_tensor* dx, tlc_tensor* dweight,
                             tlc_tensor* dbias, int accumulate, void* stream);

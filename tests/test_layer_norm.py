@@ -305,6 +305,25 @@ def test_rows_far_from_zero(d, off):
     assert (np.abs(st[..., :1] - mean) <= d_mean).all() and (np.abs(st[..., 1:] / rstd - 1) <= rel).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [16400, 20001])
+def test_sums_of_many_long_rows(d):
+    """dw and db over 100,000 rows of more than 16384 columns: x and grad are one row each, repeated, so
+    that every rounding of a running sum goes the same way."""
+    n = 100_000
+    x, _, _, g = data((1, d), d)
+    vx, vg = dev(x).expand(n, d), dev(g).expand(n, d)
+    _, stats = tlcuda.layer_norm(dev(x))
+    _, dw, db = tlcuda.layer_norm_backward(vg, vx, stats.expand(n, 2), need=(False, True, True))
+    mean, rstd = (host(stats)[0].astype(np.float64))
+    hat = (x[0].astype(np.float64) - mean) * rstd
+    # 128 rows in a running sum, a sixteenth of these 782 sums in the next, 16 in the last; 4 roundings
+    # in each product
+    adds = 128 + 49 + 16
+    for got, one, more in ((dw, g[0] * hat, 4), (db, g[0].astype(np.float64), 0)):
+        assert (np.abs(host(got) - n * one) <= (adds + more) * U * n * np.abs(one)).all()
+
+
 F = "tlc_layer_norm"
 B = "tlc_layer_norm_backward"
 A, Z = 1 << 20, 1 << 30  # addresses far apart

@@ -685,9 +685,11 @@ extern "C" int tlc_layer_norm_backward(const tlc_tensor* grad, const tlc_tensor*
         }
         if (sums) {
             const int64_t cols = ((int64_t)p.D + 255) / 256;
-            const int64_t rows_per = std::max<int64_t>(8, (p.rows * cols + 8 * sms - 1) / (8 * sms));
-            const int64_t chunks = (p.rows + rows_per - 1) / rows_per;
-            parts = (int)chunks;  // at most 8 * sms / cols + 1
+            // eight blocks an SM, but at most 128 rows in one running sum, which loses a rounding of
+            // its size with each row (as many more where the grid's 65535 block rows ask for it)
+            const int64_t even = (p.rows * cols + 8 * sms - 1) / (8 * sms);
+            const int64_t rows_per = std::max(std::clamp<int64_t>(even, 8, 128), (p.rows + 65534) / 65535);
+            parts = (int)((p.rows + rows_per - 1) / rows_per);
             TLC_TRY(scratch_alloc(&cp.p, sizeof(float) * 2 * (size_t)p.D * (size_t)parts, s));
             p.part = cp.f();
             ln_bwd_cols_kernel<<<dim3((unsigned)cols, (unsigned)parts), 256, 0, s>>>(p, rows_per);
