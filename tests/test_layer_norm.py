@@ -305,6 +305,49 @@ def test_rows_far_from_zero(d, off):
     assert (np.abs(st[..., :1] - mean) <= d_mean).all() and (np.abs(st[..., 1:] / rstd - 1) <= rel).all()
 
 
+# Rows enough that each group of threads takes more than twice as many as the gradient's ring of rows
+# has places, for every number of threads a row and of columns a thread; on 16 bytes and off them.
+MANY = [(90000, 128), (90000, 101), (60000, 256), (60000, 130), (30000, 512), (30000, 260), (25000, 768), (25000, 515),
+        (12000, 1024), (12000, 1022), (8000, 1536), (8000, 1535), (8000, 2048), (8000, 1999), (4000, 4096), (4000, 2051),
+        (1500, 6144), (1500, 5001), (2400, 8192), (1500, 8191), (1000, 12288), (1000, 10001), (1000, 16384), (1000, 16383)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", MANY, ids=str)
+def test_many_rows_a_group(shape):
+    n, d = shape
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(n + d)
+    x = torch.randn(n, d, generator=gen, device="cuda") + torch.randn(n, 1, generator=gen, device="cuda")
+    g = torch.randn(n, d, generator=gen, device="cuda") * (0.5 + torch.rand(n, 1, generator=gen, device="cuda"))
+    w = 1 + 0.3 * torch.randn(d, generator=gen, device="cuda")
+    y, stats = tlcuda.layer_norm(x, w)
+    dx, dw, db = tlcuda.layer_norm_backward(g, x, stats, w)
+    dw64, db64, dw_abs, db_abs = (torch.zeros(d, dtype=torch.float64, device="cuda") for _ in range(4))
+    for at in range(0, n, 1000):
+        part = slice(at, at + 1000)
+        xx, gg, st, ww = x[part].double(), g[part].double(), stats[part].double(), w.double()
+        hat = (xx - st[:, :1]) * st[:, 1:]
+        # the row's own statistics, and the forward with them: 4 roundings behind these
+        mean = xx.mean(-1)
+        assert ((st[:, 0] - mean).abs() <= SUM * U * xx.abs().mean(-1) + U * mean.abs()).all()
+        assert ((y[part].double() - hat * ww).abs() <= 4 * U * ((hat * ww).abs() + st[:, 1:] * ww.abs() * SUM * (
+            xx.abs().mean(-1, keepdim=True)))).all()
+        gw = gg * ww
+        ref = st[:, 1:] * (gw - gw.mean(-1, keepdim=True) - hat * (gw * hat).mean(-1, keepdim=True))
+        tol = (SUM + 10) * U * st[:, 1:] * (gw.abs() + gw.abs().mean(-1, keepdim=True)
+                                            + hat.abs() * (gw * hat).abs().mean(-1, keepdim=True))
+        assert ((dx[part].double() - ref).abs() <= tol).all(), at
+        dw64 += (gg * hat).sum(0)
+        db64 += gg.sum(0)
+        dw_abs += (gg * hat).abs().sum(0)
+        db_abs += gg.abs().sum(0)
+    # a group's rows (at most 30), a block's groups (64), a sixteenth of the blocks and the sixteen sums
+    adds = 30 + 64 + 10 + 16
+    assert ((dw.double() - dw64).abs() <= (adds + 4) * U * dw_abs).all()
+    assert ((db.double() - db64).abs() <= adds * U * db_abs).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("d", [16400, 20001])
 def test_sums_of_many_long_rows(d):

@@ -196,6 +196,43 @@ def test_ties_and_orders(V, pattern):
         check(rows, np.array([0, V - 1, V // 2]), 1.0, top)
 
 
+# More rows than the grid has warps (8000 x 200, 4000 x 3001) or blocks (1000 x 20001), so that one takes
+# several in turn; rows of several batches for a warp (1300 x 2001 to 16384).
+MANY = [(1300, 2001, 0), (1300, 2001, 5), (1300, 2001, 32), (1300, 16384, 20), (1300, 16383, 5), (4000, 3001, 0),
+        (4000, 3001, 20), (4000, 3001, 32), (8000, 200, 0), (8000, 200, 5), (8000, 200, 20), (8000, 201, 32), (1000, 20001, 0),
+        (1000, 20001, 5), (1000, 20004, 20), (1000, 20001, 32)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,V,top", MANY)
+def test_many_rows_in_turn(rows, V, top):
+    """Rows of all kinds, one after another: what one row leaves behind must not reach the next."""
+    x = logits((rows, V), rows + V)
+    rng = np.random.default_rng(V)
+    kind = rng.integers(0, 12, rows)
+    x[kind == 0] = 0.5  # all equal
+    x[kind == 1] = NINF
+    x[np.ix_(kind == 2, rng.random(V) < 0.9)] = NINF
+    few = np.flatnonzero(kind == 3)  # fewer logits than alternatives
+    x[few, :] = NINF
+    for k in range(3):
+        x[few, rng.integers(0, V, len(few))] = rng.standard_normal(len(few))
+    x[kind == 4] += 100.0
+    x[kind == 5] -= 100.0
+    x[kind == 6] = np.sort(x[kind == 6], -1)
+    t = rng.integers(-1, V, rows)
+    clean = [None if a is None else host(a) for a in check(x, t, 1.0, top)]
+    # the same with NaN in every 17th row: the others' bits stay
+    x[::17, V // 2] = np.nan
+    out = [None if a is None else host(a) for a in tlcuda.token_logprobs(dev(x), dev(t), top=top)]
+    other = np.arange(rows) % 17 != 0
+    for a, c in zip(out, clean):
+        assert a is None or np.array_equal(a[other], c[other])
+    assert np.isnan(out[1][~other]).all() and np.isnan(out[0][~other & (t >= 0)]).all()
+    if top:
+        assert np.array_equal(out[4][~other], best(x[~other], top))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("V", [100, 5000, 70001])
 def test_nan_and_infinity_stay_in_their_rows(V):
