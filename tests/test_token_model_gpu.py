@@ -217,3 +217,22 @@ def test_views_that_repeat_memory():
     assert torch.equal(tlcuda.embedding(x, t), x)
     for a, b in zip(tlcuda.token_logprobs(x, t, top=3), tlcuda.token_logprobs(x.contiguous(), t.contiguous(), top=3)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("top", [-1, -2 ** 31, 204, 2 ** 31, 2 ** 32, 2 ** 40])
+def test_alternatives_out_of_range(top):
+    """Refused before their outputs are made (2^32 wraps to 0 in an int, and would take 48 GB)."""
+    x, t = torch.zeros(1, V, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    with pytest.raises(ValueError, match="top must be 0 to the vocabulary's size"):
+        tlcuda.token_logprobs(x, t, top=top)
+    with pytest.raises(tlcuda.TLCError, match="top is at most 32"):
+        tlcuda.token_logprobs(x, t, top=33)
+    # the three other outputs, twice
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] - before <= 6
+
+
+def test_a_table_of_less_than_no_rows():
+    g, t = torch.zeros(1, 8, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="rows must not be negative"):
+        tlcuda.embedding_backward(g, t, -1)

@@ -430,7 +430,9 @@ Tensor embedding(const Tensor& weight, const Tokens& tokens, float scale) {
 
 TokenScores token_logprobs(const Tensor& logits, const Tokens& tokens, float scale, int top) {
     if (logits.sizes().empty()) throw std::invalid_argument("token_logprobs: logits must be at least 1-D");
-    if (top < 0) throw std::invalid_argument("token_logprobs: top must be 0 to the vocabulary's size");
+    if (top < 0 || top > logits.sizes().back())
+        throw std::invalid_argument("token_logprobs: top must be 0 to the vocabulary's size");
+    if (top > 32) throw std::runtime_error("token_logprobs: top is at most 32");  // as TLC_ERR_UNSUPPORTED
     const std::vector<int64_t> lead(logits.sizes().begin(), logits.sizes().end() - 1);
     auto with = [&](int64_t n) {
         std::vector<int64_t> s = lead;

@@ -57,6 +57,16 @@ static void test_errors() {
     expect_invalid([&] { tl::layer_norm(tl::Tensor(std::vector<int64_t>{}), tl::Tensor(), tl::Tensor()); }, "1-D");
     expect_invalid([&] { tl::token_logprobs(w, none); }, "empty");
     expect_invalid([&] { tl::token_logprobs(w, tl::Tokens({4}, {0, 1, 2, 0}), 1.0f, -1); }, "top");
+    // refused before any output is made
+    expect_invalid([&] { tl::token_logprobs(w, tl::Tokens({4}, {0, 1, 2, 0}), 1.0f, 4); }, "vocabulary's size");
+    expect_invalid([&] { tl::token_logprobs(w, tl::Tokens({4}, {0, 1, 2, 0}), 1.0f, 2147483647); }, "vocabulary's size");
+    bool many = false;
+    try {
+        tl::token_logprobs(tl::Tensor({1, 50}), tl::Tokens({1}, {0}), 1.0f, 33);
+    } catch (const std::runtime_error& e) {
+        many = std::string(e.what()).find("at most 32") != std::string::npos;
+    }
+    CHECK(many);
     std::cout << "errors ok\n";
 }
 

@@ -448,6 +448,9 @@ _PACK = [struct.Struct(f"=QQ{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}x")
          for n in range(MAX_DIMS + 1)]
 
 
+MAX_TOP = 32  # alternatives of token_logprobs
+
+
 def _refuse(t, dev, name, kinds):
     if t.dtype not in kinds:
         raise ValueError(f"{name}: {' or '.join(str(k)[6:] for k in kinds)}, not {t.dtype}")
@@ -591,6 +594,8 @@ def embedding_backward(grad, tokens, rows=None, scale=1.0, dweight=None, accumul
             raise ValueError("embedding_backward: accumulate needs the dweight it adds to")
         if rows is None:
             raise ValueError("embedding_backward: rows (the table's length) or dweight is needed")
+        if rows < 0:
+            raise ValueError("embedding_backward: rows must not be negative")
         dweight = _empty(grad, (rows, grad.shape[-1]))
     elif rows is not None and (dweight.dim() != 2 or rows != dweight.shape[0]):
         raise ValueError("embedding_backward: dweight has another number of rows")
@@ -617,7 +622,9 @@ def token_logprobs(logits, tokens=None, scale=1.0, top=0, need_entropy=True, nee
         entropy = _empty(logits, lead) if logp is None else _torch.empty_like(logp)
     stats = _empty(logits, (*lead, 2)) if need_stats else None
     top_logp = top_tokens = None
-    if top:
+    if not 0 <= top <= logits.shape[-1]:  # an int of the C ABI would wrap
+        raise ValueError("token_logprobs: top must be 0 to the vocabulary's size")
+    if 0 < top <= MAX_TOP:  # more are refused below
         lead = (*lead, top)
         top_logp = _empty(logits, lead)
         top_tokens = _empty(logits, lead, _torch.int64 if tokens is None else tokens.dtype)
