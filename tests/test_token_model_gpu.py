@@ -236,3 +236,18 @@ def test_a_table_of_less_than_no_rows():
     g, t = torch.zeros(1, 8, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
     with pytest.raises(ValueError, match="rows must not be negative"):
         tlcuda.embedding_backward(g, t, -1)
+
+
+def test_views_that_torch_negates_lazily():
+    """The imaginary part of a conjugate holds the values' negatives and a mark that says so: what is
+    behind its address is not what it means."""
+    x = torch.randn(6, 40, dtype=torch.complex64, device="cuda").conj().imag
+    assert x.is_neg() and x.dtype is torch.float32
+    y, st = tlcuda.layer_norm(x.resolve_neg())
+    t = torch.arange(6, device="cuda")
+    for call in (lambda: tlcuda.layer_norm(x), lambda: tlcuda.layer_norm(y, None, x[0]),
+                 lambda: tlcuda.layer_norm_backward(x, y, st), lambda: tlcuda.embedding(x, t),
+                 lambda: tlcuda.embedding_backward(x, t, 6), lambda: tlcuda.token_logprobs(x, t),
+                 lambda: tlcuda.token_logprobs_backward(y, t, st, x[:, 0])):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()

@@ -456,7 +456,9 @@ def _refuse(t, dev, name, kinds):
         raise ValueError(f"{name}: {' or '.join(str(k)[6:] for k in kinds)}, not {t.dtype}")
     if t.dim() > MAX_DIMS:
         raise ValueError(f"{name}: at most {MAX_DIMS} dims")
-    raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+    raise ValueError(f"{name}: a view whose values torch has yet to negate (call resolve_neg() first)")
 
 
 def _fview(t, dev, name):
@@ -464,7 +466,7 @@ def _fview(t, dev, name):
     if t is None:
         return None
     n = t.dim()
-    if t.dtype is not _torch.float32 or not t.is_cuda or t.get_device() != dev or n > MAX_DIMS:
+    if t.dtype is not _torch.float32 or t.get_device() != dev or n > MAX_DIMS or t.is_neg():
         _refuse(t, dev, name, (_torch.float32,))
     return _PACK[n](t.data_ptr(), n, *t.shape, *t.stride())
 
@@ -475,7 +477,7 @@ def _iview(t, dev, name):
         return None
     n = t.dim()
     bits = 64 if t.dtype is _torch.int64 else 32
-    if (bits == 32 and t.dtype is not _torch.int32) or not t.is_cuda or t.get_device() != dev or n > MAX_DIMS:
+    if (bits == 32 and t.dtype is not _torch.int32) or t.get_device() != dev or n > MAX_DIMS:
         _refuse(t, dev, name, (_torch.int32, _torch.int64))
     return _PACK[n](t.data_ptr(), n | bits << 32, *t.shape, *t.stride())
 
@@ -484,12 +486,12 @@ _torch = None
 
 
 def _device(x):
-    """The current CUDA device (-1, which no tensor is on, where `x` is on none)."""
+    """The current CUDA device (-2, which no tensor is on, where `x` is on none)."""
     global _torch
     if _torch is None:
         import torch
         _torch = torch
-    return _torch.cuda.current_device() if x.is_cuda else -1
+    return _torch.cuda.current_device() if x.is_cuda else -2
 
 
 def _on_stream(f):
