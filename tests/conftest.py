@@ -14,6 +14,13 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA (B200) device")
 
 
+def pytest_collection_modifyitems(items):
+    """Without the reference library's build (oracle/_ref) the benchmark line's test cannot pass: it comes
+    last then, so that a run that stops at the first failure has run all others."""
+    if not os.path.exists(os.path.join(REPO, "oracle", "_ref")):
+        items.sort(key=lambda item: item.name == "test_our_arm_line")
+
+
 @pytest.fixture(scope="session")
 def golden():
     import numpy as np
