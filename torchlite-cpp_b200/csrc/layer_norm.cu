@@ -121,8 +121,9 @@ __global__ void __launch_bounds__(THREADS <= 32 ? 128 : THREADS, THREADS <= 32 ?
 }
 
 // Rows too long for the registers of a block (above 32768 columns, 16384
-// unaligned): the row is read three times (from L2 after the first).
-__global__ void __launch_bounds__(1024) ln_fwd_long_kernel(LnFwd p) {
+// unaligned): the row is read three times (from L2 after the first).  Two blocks
+// an SM read while one another's sums meet (4096 x 40000 445 us, one block 482).
+__global__ void __launch_bounds__(1024, 2) ln_fwd_long_kernel(LnFwd p) {
     __shared__ float red[32], red2[64];
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const float* xr = p.x + p.xm.offset(r);
