@@ -331,7 +331,10 @@ int tlc_flash_attention_backward(const tlc_tensor* grad_out, const tlc_tensor* q
 /* y = (x - mean) rstd * weight + bias over the last dim D of x, with
  * rstd = 1 / sqrt(var + eps) and var = sum (x - mean)^2 / D.  weight and bias:
  * NULL or [D].  stats: NULL or [..., 2], receives (mean, rstd) of each row:
- * what the backward needs.  eps must be finite and >= 0. */
+ * what the backward needs.  eps must be finite and >= 0 (0: a row of one value has
+ * no result that means anything).  A first mean is corrected by the mean of the
+ * differences to it, so rows far from zero lose nothing but the rounding of the
+ * mean in stats (2^-24 |mean| rstd in the backward's xhat). */
 int tlc_layer_norm(const tlc_tensor* x, const tlc_tensor* weight, const tlc_tensor* bias, float eps,
                    tlc_tensor* out, tlc_tensor* stats, void* stream);
 /* The gradients from grad (x's shape), x, the forward's stats and weight
@@ -359,8 +362,10 @@ int tlc_embedding(const tlc_tensor* weight, const tlc_index* tokens, float scale
  * zeros for tokens that do not occur; with accumulate != 0 these sums are
  * added to what dweight holds (rows that do not occur stay as they are).
  * Tokens outside [0, V), -1 among them, take no part.  The positions are
- * sorted by token, so each row's additions have one fixed order.  Takes
- * scratch of an eighth of grad's size at most (two rows at least) and 20 bytes a position from the
+ * sorted by token, so each row's additions have one fixed order: running sums over
+ * at most 32 positions, then over at most 17 of these, or an eighth of them for a
+ * token in hundreds of positions, and the eight.  Takes scratch of at most
+ * 2 ceil(positions / 16) rows of D floats, 20 bytes a position and 32 from the
  * device's memory pool; at most 2^31 - 8193 positions and 2^31 - 2 rows
  * (TLC_ERR_UNSUPPORTED). */
 int tlc_embedding_backward(const tlc_tensor* grad, const tlc_index* tokens, float scale,
@@ -379,7 +384,10 @@ int tlc_embedding_backward(const tlc_tensor* grad, const tlc_index* tokens, floa
  * Token -1: none is asked for, logprobs 0 (the row's other results as usual);
  * any other token outside [0, V): NaN.  A row of -inf alone has no
  * distribution: log-probabilities -inf, entropy 0.  A NaN or +inf in a row
- * makes its results NaN; NaN ranks above every number in top_tokens. */
+ * makes its results NaN (but for token -1's 0); NaN ranks above every number in
+ * top_tokens.  A probability below 2^-126 counts as 0, and so does one whose
+ * logit's difference to the largest leaves float32.  Sums: a running sum over one
+ * in 64 of a row's values (rows of at most 16384) or one in 512, then trees. */
 int tlc_token_logprobs(const tlc_tensor* logits, const tlc_index* tokens, float scale,
                        tlc_tensor* logprobs, tlc_tensor* entropy, tlc_tensor* stats, int top,
                        tlc_tensor* top_logprobs, tlc_index* top_tokens, void* stream);
@@ -387,8 +395,8 @@ int tlc_token_logprobs(const tlc_tensor* logits, const tlc_index* tokens, float 
  *   dlogits_j = scale (g (1[j = token] - p_j) - h p_j (log p_j + entropy)),
  * with the forward's stats and, with grad_entropy, its entropy.  The gradients
  * may be broadcast views (stride 0).  No gradient flows from top_logprobs, from
- * the log-probability of token -1, or into a row of -inf alone; a token that
- * gave NaN gives a row of NaN.  dlogits may be the memory of (contiguous)
+ * the log-probability of token -1, or into a row of -inf alone (whatever its
+ * token); elsewhere a token that gave NaN gives a row of NaN.  dlogits may be the memory of (contiguous)
  * logits. */
 int tlc_token_logprobs_backward(const tlc_tensor* logits, const tlc_index* tokens,
                                 const tlc_tensor* stats, const tlc_tensor* entropy,

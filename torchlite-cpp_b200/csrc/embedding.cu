@@ -16,7 +16,10 @@
 // gradient reads 4 an element of g and writes 4 an element of the table.
 // Measured (GPU time): lookup 32768 x 4096 of 131072 rows 117 us (6.0 TB/s),
 // 131072 x 64 9.3 us; gradient 65536 x 2048 into 100003 rows 244 us (5.5
-// TB/s), 8192 x 768 into 32000 33 us (3.5 TB/s: three dependent kernels).
+// TB/s), 8192 x 768 into 32000 33 us (3.5 TB/s: three dependent kernels).  Many
+// short rows are bound by the sort on eight SMs: 131072 x 64 into 1000 rows 64 us,
+// 1048576 x 64 into 32000 471 us; so is accumulation (8192 x 768 27 us, 65536 x
+// 2048 228 us), where no zeros are written beside it.
 #include <algorithm>
 #include <cmath>
 
@@ -721,7 +724,7 @@ extern "C" int tlc_embedding_backward(const tlc_tensor* grad, const tlc_index* t
     const bool vec = D % 4 == 0 && vg.map.multiple_of(4) && aligned_to(vg.data, 16) && aligned_to(dweight->data, 16);
     // 32 positions a chunk; 16 where that would leave an SM fewer than 16 warps
     const int64_t slices = (D + 255) / 256;
-    const int ch = (n / 32) * slices >= 148 * 16 ? 32 : 16;
+    const int ch = (n / 32) * slices >= (int64_t)sm_count() * 16 ? 32 : 16;
     const int64_t chunks = (n + ch - 1) / ch;
     // one workspace: the parts, the two lists, the crossing runs
     const size_t part_bytes = sizeof(float) * 2 * (size_t)chunks * (size_t)D;

@@ -46,8 +46,9 @@ struct LnFwd {
 };
 
 // THREADS threads a row (a block, or up to 32 neighbouring lanes of 4 warps), VPT
-// vectors of VEC floats a thread: D <= THREADS * VPT * VEC.  64 registers a
-// thread, so that 1024 threads are on an SM.
+// vectors of VEC floats a thread: D <= THREADS * VPT * VEC.  Blocks that share a row
+// have 64 registers a thread, so that 1024 threads are on an SM; the lane groups, whose
+// blocks hold several rows, are not bounded (62 to 85).
 template <int VEC, int VPT, int THREADS>
 __global__ void __launch_bounds__(THREADS <= 32 ? 128 : THREADS, THREADS <= 32 ? 1 : 1024 / THREADS)
     ln_fwd_kernel(LnFwd p) {
