@@ -69,7 +69,8 @@ def build(jobs: int = 8, verbose: bool = False, ptxas_info: bool = False) -> dic
 
     # C++ tl:: layer over the C ABI.
     host_src = sorted(glob.glob(os.path.join(PKG, "host", "src", "*.cpp")))
-    host_hdr = sorted(glob.glob(os.path.join(PKG, "host", "include", "tl", "*.h")))
+    host_hdr = sorted(glob.glob(os.path.join(PKG, "host", "include", "tl", "*.h")) +
+                      glob.glob(os.path.join(PKG, "host", "src", "*.h")))
     tl_so = os.path.join(LIB, "libtorchlite_b200.so")
     if host_src and _stale(tl_so, host_src + host_hdr + [so]):
         _run(["g++"] + CXX_FLAGS + ["-shared", "-o", tl_so] + host_src +

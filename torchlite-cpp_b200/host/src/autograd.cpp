@@ -7,6 +7,8 @@
 #include <stdexcept>
 #include <string>
 
+#include "token_view.h"
+
 namespace tl {
 
 namespace {
@@ -36,20 +38,6 @@ tlc_tensor hview(const Tensor& t) {
         v.strides[i] = t.strides()[i];
     }
     v.data = t.numel() > 0 ? const_cast<float*>(t.data()) : nullptr;
-    return v;
-}
-
-tlc_index iview(const Tokens& t) {
-    tlc_index v{};
-    v.ndim = static_cast<int32_t>(t.sizes().size());
-    v.bits = 64;
-    int64_t step = 1;
-    for (int i = v.ndim - 1; i >= 0; --i) {
-        v.sizes[i] = t.sizes()[i];
-        v.strides[i] = step;
-        step *= t.sizes()[i];
-    }
-    v.data = t.numel() > 0 ? const_cast<int64_t*>(t.device_data()) : nullptr;
     return v;
 }
 
@@ -242,7 +230,7 @@ void EmbeddingBackward::backward(const Tensor& grad_output) {
     if (!inputs[0].requires_grad) return;
     Tensor dw = Tensor::device_empty(weight_sizes);
     tlc_tensor g = dview(grad_output), vd = dview(dw);
-    tlc_index t = iview(tokens);
+    tlc_index t = index_of(tokens);
     check(tlc_embedding_backward(&g, &t, scale, &vd, 0, nullptr), "tlc_embedding_backward");
     accumulate_grad(inputs[0], dw);
 }
@@ -252,7 +240,7 @@ void TokenLogprobsBackward::backward(const Tensor& grad_output) {
     Tensor dx = Tensor::device_empty(logits_cache.sizes());
     tlc_tensor x = dview(logits_cache), st = dview(stats_cache), g = dview(grad_output), vd = dview(dx), h{};
     if (of_entropy) h = dview(entropy_cache);
-    tlc_index t = iview(tokens);
+    tlc_index t = index_of(tokens);
     check(tlc_token_logprobs_backward(&x, &t, &st, of_entropy ? &h : nullptr, of_entropy ? nullptr : &g,
                                       of_entropy ? &g : nullptr, scale, &vd, nullptr),
           "tlc_token_logprobs_backward");

@@ -14,6 +14,8 @@
 #include <string>
 #include <vector>
 
+#include "token_view.h"
+
 namespace tl {
 
 namespace {
@@ -363,22 +365,6 @@ Tensor flash_attention(const Tensor& Q, const Tensor& K, const Tensor& V, float 
 }
 
 namespace {
-
-tlc_index index_of(const Tokens& t) {
-    if (t.empty()) throw std::invalid_argument("Tokens: empty");
-    if (t.sizes().size() > TLC_MAX_DIMS) throw std::invalid_argument("Tokens: more than 8 dims");
-    tlc_index v{};
-    v.ndim = static_cast<int32_t>(t.sizes().size());
-    v.bits = 64;
-    int64_t step = 1;
-    for (int i = v.ndim - 1; i >= 0; --i) {
-        v.sizes[i] = t.sizes()[i];
-        v.strides[i] = step;
-        step *= t.sizes()[i];
-    }
-    v.data = t.numel() > 0 ? const_cast<int64_t*>(t.device_data()) : nullptr;
-    return v;
-}
 
 // The view of a result that the call writes on the device.
 tlc_tensor out_view(Tensor& t) {
