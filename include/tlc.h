@@ -334,7 +334,9 @@ int tlc_flash_attention_backward(const tlc_tensor* grad_out, const tlc_tensor* q
  * what the backward needs.  eps must be finite and >= 0 (0: a row of one value has
  * no result that means anything).  A first mean is corrected by the mean of the
  * differences to it, so rows far from zero lose nothing but the rounding of the
- * mean in stats (2^-24 |mean| rstd in the backward's xhat). */
+ * mean in stats (2^-24 |mean| rstd in the backward's xhat).  A row with NaN or
+ * infinities gives NaN (an infinite mean stays in stats), one whose sum or sum of
+ * squares leaves float32 what infinite sums give. */
 int tlc_layer_norm(const tlc_tensor* x, const tlc_tensor* weight, const tlc_tensor* bias, float eps,
                    tlc_tensor* out, tlc_tensor* stats, void* stream);
 /* The gradients from grad (x's shape), x, the forward's stats and weight

@@ -203,6 +203,19 @@ def test_values_at_the_edges():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [7, 300, 1000, 5001, 8192, 40000])
+def test_means_that_are_not_finite(d):
+    """stats holds the mean that the row has: infinite with infinities of one sign, NaN with both or a NaN."""
+    inf, nan = float("inf"), float("nan")
+    x = torch.randn(5, d, device="cuda")
+    x[0, d // 2], x[1, 0], x[2, d - 1], x[3, 1], x[3, 2] = inf, -inf, nan, inf, -inf
+    y, stats = tlcuda.layer_norm(x)
+    assert stats[0, 0] == inf and stats[1, 0] == -inf and torch.isnan(stats[2:4, 0]).all()
+    assert torch.isnan(stats[:4, 1]).all() and torch.isnan(y[:4]).all()
+    assert torch.isfinite(stats[4]).all() and torch.isfinite(y[4]).all()
+
+
+@pytest.mark.gpu
 def test_no_rows():
     w = torch.ones(16, device="cuda")
     y, stats = tlcuda.layer_norm(torch.empty(0, 16, device="cuda"), w, w)

@@ -34,6 +34,11 @@ struct Spread {
         rstd = __frsqrt_rn((var < 0.0f ? 0.0f : var) + eps);  // a NaN stays one
         shift = -off * rstd;
     }
+    // the corrected mean; an infinite one, whose differences are infinite too, stays
+    __device__ __forceinline__ float mean(float first) const {
+        const float m = first + off;
+        return m == m ? m : first;
+    }
 };
 
 struct LnFwd {
@@ -88,7 +93,7 @@ __global__ void __launch_bounds__(THREADS <= 32 ? 128 : THREADS, THREADS <= 32 ?
         group_sum<THREADS, FEW>(d, red2);
         const Spread sp(d, p.D, p.eps);
         if (p.stats && t == 0 && live) {
-            p.stats[2 * r] = mean + sp.off;
+            p.stats[2 * r] = sp.mean(mean);
             p.stats[2 * r + 1] = sp.rstd;
         }
         float* yr = p.out + r * p.D + t * VEC;
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(1024, 2) ln_fwd_long_kernel(LnFwd p) {
             yr[j] = y;
         }
         if (p.stats && threadIdx.x == 0) {
-            p.stats[2 * r] = mean + sp.off;
+            p.stats[2 * r] = sp.mean(mean);
             p.stats[2 * r + 1] = sp.rstd;
         }
     }
